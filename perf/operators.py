@@ -242,7 +242,7 @@ def _own(s):
                   ptr(s["dgate"]), ptr(s["dup"]), ptr(s["act"]), rows, D, st)
         return {"dgate": s["dgate"], "dup": s["dup"], "act": s["act"]}
     _ctx.call("ta_gemm_tokens_q8_f32", s["M"], D, rows, s["alpha"], ptr(s["dh"]), s["M"], ptr(s["q"]), ptr(s["scale"]), ptr(s["col"]),
-              ptr(s["gA"]), D, 0, None, 0, st)
+              ptr(s["gA"]), D, 0, st)
     return {"gA": s["gA"]}
 
 
