@@ -190,6 +190,50 @@ int ta_swiglu_proj_fwd(ta_ctx* ctx, const void* x, const void* gate_w, const voi
 int ta_swiglu_down_bwd(ta_ctx* ctx, const void* dY, const void* down_w, const void* dh, const void* A_down, const void* gate,
                        const void* up, void* d_gate, void* d_up, int BT, int hidden, int inter, int rank, void* stream);
 
+/* ── activations in 8 bits ─────────────────────────────────────────────────────────────────
+ * What the forward keeps for the backward takes most of the device's memory (the reference keeps every activation in BF16,
+ * src/base/arch/qwen2.cu:47-160).  These entry points keep it in 8 bits and let the backward read it from there; the
+ * reference has no counterpart.  An 8-bit activation of [rows, D] BF16 values is two device arrays of the caller:
+ *     q      [rows][D]                    e4m3 (1 sign, 4 exponent, 3 fraction bits; 448 is the largest value)
+ *     scale  [rows][(D + 31) / 32]        one byte b per row and TA_Q8_BLOCK columns: value = q * 2^(b - 127)
+ * b - 127 is the smallest whole number k with amax <= 448 * 2^k, amax over the block's finite elements, kept in [-117, 119]
+ * (magnitudes above 448 * 2^119 = 2.97e38 come out as that).  A value is off by at most half a step of e4m3: 2^-4 of itself, or
+ * 2^(k-10) where it is below 2^(k-6); every value is exact in BF16.  An infinity or NaN is held as NaN, the other elements of
+ * its block as they would be without it.  D is any multiple of 8; q is 16-byte aligned, scale needs no alignment.
+ * All calls take contiguous rows and allocate nothing (so they can be captured into a graph); the context's device must be
+ * the current device.  An output may be the same array as a BF16 input where that is said, and may not overlap one otherwise. */
+#define TA_Q8_BLOCK 32
+/* x [rows, D] BF16 into 8 bits, and back: out = bf16(value * col[column]); col [D] BF16 or NULL (then out is exact). */
+int ta_q8_store(ta_ctx* ctx, const void* x, void* q, void* scale, int rows, int D, void* stream);
+int ta_q8_load(ta_ctx* ctx, const void* q, const void* scale, const void* col, void* out, int rows, int D, void* stream);
+/* The residual add and the norm that follows it (ops::add_inplace, ops.hpp:121-126, then ops::rms_norm_fwd, ops.hpp:12-18) in
+ * one pass that also leaves the normalised rows in 8 bits:
+ *     res_out = bf16(x + delta)    n = res_out / rms(res_out)    out = bf16(n * w)    (q, scale) = n in 8 bits
+ * rms_out [rows] receives 1 / sqrt(mean(res_out^2) + eps), as in ta_rms_norm_fwd.  delta NULL: no addition, res_out (which may
+ * then be NULL) is a copy of x.  out may be NULL.  res_out and out may be x or delta, not one another.  n is held and not n * w:
+ * the norm's backward needs n, and ta_q8_load / ta_gemm_tokens_q8_f32 take w as `col`.  D <= 16384. */
+int ta_add_rms_norm_q8_fwd(ta_ctx* ctx, const void* x, const void* delta, const void* w, void* res_out, void* out, void* q, void* scale,
+                           float* rms_out, int rows, int D, float eps, void* stream);
+/* ta_rms_norm_bwd from the 8 bits that ta_add_rms_norm_q8_fwd left:
+ *     dx = bf16((add_to +) rms * (w*dy - n * mean(w*dy*n)))        rounded once, also with add_to
+ * add_to may be NULL; dx may be dy or add_to.  D <= 16384. */
+int ta_rms_norm_q8_bwd(ta_ctx* ctx, const void* dy, const void* q, const void* scale, const void* w, const float* rms_saved, void* dx,
+                       const void* add_to, int rows, int D, void* stream);
+/* ta_silu_mul_fwd that also leaves gate and up in 8 bits (out itself is formed from the BF16 values); out may be gate or up. */
+int ta_silu_mul_q8_fwd(ta_ctx* ctx, const void* gate, const void* up, void* out, void* gate_q, void* gate_scale, void* up_q, void* up_scale,
+                       int rows, int D, void* stream);
+/* ta_silu_mul_bwd from those 8 bits; act, if not NULL, receives bf16(silu(gate) * up) of the 8-bit values again, which the
+ * gradient of the down projection's adapter needs, so the forward need not keep it.  One of dgate, dup, act may be dout. */
+int ta_silu_mul_q8_bwd(ta_ctx* ctx, const void* dout, const void* gate_q, const void* gate_scale, const void* up_q, const void* up_scale,
+                       void* dgate, void* dup, void* act, int rows, int D, void* stream);
+/* ta_gemm_tokens_f32 for an adapter's gA with the input in 8 bits:
+ *     C[M,N] (+)= alpha * col[n] * sum_k A[k][m] * value[k][n]
+ * A [K][lda] BF16 (dh, of one adapter or of several that share the input), q / scale [K][N] as above, col [N] BF16 or NULL,
+ * C FP32 row-major with pitch ldc, added to if accumulate != 0.  M, N and lda multiples of 8; K may be 0.  Sums in FP32, in an
+ * order that depends on M, N and K alone: the same bits every time. */
+int ta_gemm_tokens_q8_f32(ta_ctx* ctx, int M, int N, int K, float alpha, const void* A, long lda, const void* q, const void* scale,
+                          const void* col, float* C, long ldc, int accumulate, void* stream);
+
 /* ── attention ─────────────────────────────────────────────────────────────────────────────
  * ops::sdpa_fwd / ops::sdpa_bwd (ops.hpp:52-70, src/backend/cuda/ops.cu:578-907): causal GQA
  * attention, scale 1/sqrt(head_dim), Q/out [B*T, Hq*hd], K/V [B*T, Hkv*hd]. Instead of the

@@ -71,6 +71,13 @@ _PROTOS = {
     "ta_trainer_set_option": (c_int, [P, c_char_p, c_int]),
     "ta_lora_linear_fwd": (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_float, P]),
     "ta_lora_linear_bwd": (c_int, [P, P, P, P, P, P, P, c_int, P, P, c_int, c_int, c_int, c_int, c_float, P]),
+    "ta_q8_store": (c_int, [P, P, P, P, c_int, c_int, P]),
+    "ta_q8_load": (c_int, [P, P, P, P, P, c_int, c_int, P]),
+    "ta_add_rms_norm_q8_fwd": (c_int, [P, P, P, P, P, P, P, P, P, c_int, c_int, c_float, P]),
+    "ta_rms_norm_q8_bwd": (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, P]),
+    "ta_silu_mul_q8_fwd": (c_int, [P, P, P, P, P, P, P, P, c_int, c_int, P]),
+    "ta_silu_mul_q8_bwd": (c_int, [P, P, P, P, P, P, P, P, P, c_int, c_int, P]),
+    "ta_gemm_tokens_q8_f32": (c_int, [P, c_int, c_int, c_int, c_float, P, c_long, P, P, P, P, c_long, c_int, P]),
     "ta_flash_attn_fwd": (c_int, [P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
     "ta_flash_attn_bwd": (c_int, [P, P, P, P, P, P, P, P, P, P, P, c_int, c_int, c_int, c_int, c_int, P]),
     "ta_sum_sq_into": (c_int, [P, P, P, c_long, P]),

@@ -16,6 +16,13 @@ int check_cuda(ta_ctx* ctx, cudaError_t e, const char* what) {
     return fail(ctx, TA_ERR_CUDA, std::string(what) + ": " + cudaGetErrorString(e));
 }
 
+int on_ctx_device(ta_ctx* ctx, const char* what) {
+    int dev = -1;
+    TA_CUDA(ctx, cudaGetDevice(&dev));
+    if (dev != ctx->device) return fail(ctx, TA_ERR_INVALID, std::string(what) + ": the context's device must be the current device");
+    return TA_OK;
+}
+
 using EncodeTiledFn = CUresult (*)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*,
                                    const cuuint64_t*, const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave,
                                    CUtensorMapSwizzle, CUtensorMapL2promotion, CUtensorMapFloatOOBfill);

@@ -78,6 +78,8 @@ namespace ta {
 
 int fail(ta_ctx* ctx, int code, const std::string& msg);
 int check_cuda(ta_ctx* ctx, cudaError_t e, const char* what);
+// TA_ERR_INVALID unless the context's device is the current one (a launch goes to the current device).
+int on_ctx_device(ta_ctx* ctx, const char* what);
 
 // Cached 2-D BF16 tensor map: tensor [dim1 rows][dim0 cols], row pitch in bytes, box [box1 rows][box0 cols], swizzle
 // matching the box's inner extent (128 B for 64 columns, 64 B for 32); out-of-bounds elements read as zero and are not
