@@ -39,8 +39,8 @@ static EncodeTiledFn encode_fn() {
     return fn;
 }
 
-int encode_tmap_bf16(ta_ctx* ctx, const void* ptr, uint64_t dim0, uint64_t dim1, uint64_t pitch_bytes, uint32_t box0,
-                     uint32_t box1, CUtensorMap* out) {
+int encode_tmap_2d(ta_ctx* ctx, CUtensorMapDataType type, const void* ptr, uint64_t dim0, uint64_t dim1, uint64_t pitch_bytes,
+                   uint32_t box0, uint32_t box1, int span, CUtensorMap* out) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return fail(ctx, TA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
     if ((reinterpret_cast<uintptr_t>(ptr) & 15) || (pitch_bytes & 15))
@@ -49,12 +49,10 @@ int encode_tmap_bf16(ta_ctx* ctx, const void* ptr, uint64_t dim0, uint64_t dim1,
     cuuint64_t gstride[1] = {pitch_bytes};
     cuuint32_t box[2] = {box0, box1};
     cuuint32_t estr[2] = {1, 1};
-    // swizzle = the inner extent of the box: 64 elements (128 B) for the MMA operand tiles, 32 elements (64 B) for the
-    // 32 x 32 output tiles the GEMM epilogue stores
-    const CUtensorMapSwizzle swz = box0 >= 64 ? CU_TENSOR_MAP_SWIZZLE_128B : box0 == 32 ? CU_TENSOR_MAP_SWIZZLE_64B : CU_TENSOR_MAP_SWIZZLE_NONE;
-    CUresult r = fn(out, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(ptr), gdim, gstride, box, estr,
-                    CU_TENSOR_MAP_INTERLEAVE_NONE, swz, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
-                    CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    const CUtensorMapSwizzle swz = span == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : span == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
+                                 : span == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_NONE;
+    CUresult r = fn(out, type, 2, const_cast<void*>(ptr), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
+                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         char buf[200];
         std::snprintf(buf, sizeof(buf), "cuTensorMapEncodeTiled failed (%d) dims=%llu x %llu pitch=%llu box=%u x %u",
@@ -63,6 +61,13 @@ int encode_tmap_bf16(ta_ctx* ctx, const void* ptr, uint64_t dim0, uint64_t dim1,
         return fail(ctx, TA_ERR_CUDA, buf);
     }
     return TA_OK;
+}
+
+int encode_tmap_bf16(ta_ctx* ctx, const void* ptr, uint64_t dim0, uint64_t dim1, uint64_t pitch_bytes, uint32_t box0,
+                     uint32_t box1, CUtensorMap* out) {
+    // swizzle = the inner extent of the box: 64 elements (128 B) for the MMA operand tiles, 32 elements (64 B) for the
+    // 32 x 32 output tiles the GEMM epilogue stores
+    return encode_tmap_2d(ctx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, ptr, dim0, dim1, pitch_bytes, box0, box1, box0 >= 64 ? 128 : box0 == 32 ? 64 : 0, out);
 }
 
 int get_tmap_bf16(ta_ctx* ctx, const void* ptr, uint64_t dim0, uint64_t dim1, uint64_t pitch_bytes, uint32_t box0,
