@@ -109,7 +109,19 @@ __global__ void __launch_bounds__(kThreads) q8_load_kernel(Rows r, const uint2* 
     }
 }
 
-// act = silu(gate) * up; gate and up to 8 bits.  12 + 2/32 ... 8 + 1/16 bytes an element, read once and written once.
+// 1 / (1 + 2^(-g log2 e)) by the special-function unit: relative error under 8 + 1.5 |g| halves of FP32's step (the product's
+// rounding is |g| of them, its constant half as many, ex2 and rcp four each), and at -88 and below, where the sum passes FLT_MAX,
+// zero for at most 2^-127.  The results are rounded to BF16's 2^-8 next.  expf and a division instead make the kernels below bound
+// by instructions: 448 against 363 us forward, 508 against 465 backward, at 16384 x 18944.
+__device__ __forceinline__ float sigmoid(float g) {
+    float e, r;
+    asm("ex2.approx.f32 %0, %1;" : "=f"(e) : "f"(g * -1.4426950408889634f));
+    asm("rcp.approx.f32 %0, %1;" : "=f"(r) : "f"(1.f + e));
+    return r;
+}
+
+// act = silu(gate) * up; gate and up to 8 bits: 4 bytes an element read, 4 + 1/16 written.  Two vectors a thread: with one the
+// loads in flight do not cover the latency (419 us), four cost registers (385 us).
 template <bool RAGGED, int U>
 __global__ void __launch_bounds__(kThreads) silu_mul_q8_fwd_kernel(Rows r, const uint4* gate, const uint4* up, uint4* act, uint2* gate_q,
                                                                    uint8_t* gate_s, uint2* up_q, uint8_t* up_s) {
@@ -130,7 +142,7 @@ __global__ void __launch_bounds__(kThreads) silu_mul_q8_fwd_kernel(Rows r, const
         int bg, bu;
         const uint2 qg = narrow8(fg, bg), qu = narrow8(fu, bu);
 #pragma unroll
-        for (int e = 0; e < 8; e++) a[e] = fg[e] / (1.f + expf(-fg[e])) * fu[e];
+        for (int e = 0; e < 8; e++) a[e] = fg[e] * sigmoid(fg[e]) * fu[e];
         if (p[u].on) {
             act[p[u].vec] = pack8(a);
             gate_q[p[u].vec] = qg;
@@ -170,7 +182,7 @@ __global__ void __launch_bounds__(kThreads) silu_mul_q8_bwd_kernel(Rows r, const
         widen8(h[u], bu[u], fu);
 #pragma unroll
         for (int e = 0; e < 8; e++) {
-            const float sig = 1.f / (1.f + expf(-fg[e])), s = fg[e] * sig;
+            const float sig = sigmoid(fg[e]), s = fg[e] * sig;
             og[e] = fd[e] * fu[e] * (sig * (1.f + fg[e] * (1.f - sig)));
             ou[e] = fd[e] * s;
             oa[e] = s * fu[e];
@@ -182,8 +194,10 @@ __global__ void __launch_bounds__(kThreads) silu_mul_q8_bwd_kernel(Rows r, const
 }
 
 // ── RMSNorm ─────────────────────────────────────────────────────────────────
-// A row belongs to TPR threads (a warp, or a whole CTA of 128 or 256), which hold it in registers: one read.  A lane has
-// NV vectors of 8 columns, TPR vectors apart, so the four lanes of a block of 32 columns are neighbours.
+// A row belongs to TPR threads (a warp, four of which make a CTA, or a whole CTA), which hold it in registers: one read.  A thread
+// has NV vectors of 8 columns, TPR vectors apart, so the four lanes of a block of 32 columns are neighbours.  Many small CTAs: one
+// row's barrier and latencies are covered by the other rows on the SM, two or four rows a CTA are slower (67 / 83 us backward at
+// 16384 x 3584, a warp a row 100).  All loads of a row stand before its sum, add_to's too (after it: 77 us).
 //
 // Sum over the threads of a row; every thread gets it.  A warp's sum needs no barrier; a CTA's one.
 template <int TPR>
@@ -202,10 +216,10 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 // r = bf16(x + delta), n = r / rms(r), out = bf16(n * w), (q, scale) = n in 8 bits.  n and not n * w is held: the backward
 // needs n, and a gradient over tokens of out = n * w has w as a factor of its columns (ta_gemm_tokens_q8_f32's `col`).
 template <int TPR, int NV>
-__global__ void __launch_bounds__(TPR < 256 ? 128 : 256) add_rms_norm_q8_fwd_kernel(const uint4* x, const uint4* delta, const uint4* __restrict__ w,
+__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) add_rms_norm_q8_fwd_kernel(const uint4* x, const uint4* delta, const uint4* __restrict__ w,
                                                                                     uint4* res, uint4* out, uint2* q, uint8_t* scale,
                                                                                     float* rms_out, int rows, int D, float eps) {
-    __shared__ float red[8];
+    __shared__ float red[TPR / 32];
     const int lane = threadIdx.x % TPR;
     const int row = TPR == 32 ? blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
     if (row >= rows) return;   // a whole warp's, or a whole CTA's
@@ -278,18 +292,18 @@ __global__ void __launch_bounds__(TPR < 256 ? 128 : 256) add_rms_norm_q8_fwd_ker
 
 // dx = rms * (w*dy - n * mean(w*dy*n)) (+ add_to), n from 8 bits
 template <int TPR, int NV>
-__global__ void __launch_bounds__(TPR < 256 ? 128 : 256) rms_norm_q8_bwd_kernel(const uint4* dy, const uint2* __restrict__ q,
+__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) rms_norm_q8_bwd_kernel(const uint4* dy, const uint2* __restrict__ q,
                                                                                 const uint8_t* __restrict__ scale, const uint4* __restrict__ w,
                                                                                 const float* __restrict__ rms_saved, uint4* dx,
                                                                                 const uint4* add_to, int rows, int D) {
-    __shared__ float red[8];
+    __shared__ float red[TPR / 32];
     const int lane = threadIdx.x % TPR;
     const int row = TPR == 32 ? blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
     if (row >= rows) return;
     const int nvec = D / 8, nblk = (D + kQ8Block - 1) / kQ8Block;
     const size_t at = size_t(row) * nvec;
     const float rms = rms_saved[row];
-    uint4 d[NV];
+    uint4 d[NV], a[NV];
     uint2 n[NV];
     int b[NV];
 #pragma unroll
@@ -299,6 +313,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 128 : 256) rms_norm_q8_bwd_kernel(
         d[j] = on ? dy[at + i] : make_uint4(0, 0, 0, 0);
         n[j] = on ? q[at + i] : make_uint2(0, 0);
         b[j] = on ? scale[size_t(row) * nblk + (i >> 2)] : 127;
+        a[j] = on && add_to ? add_to[at + i] : make_uint4(0, 0, 0, 0);
     }
     float dot = 0.f;
 #pragma unroll
@@ -326,7 +341,7 @@ __global__ void __launch_bounds__(TPR < 256 ? 128 : 256) rms_norm_q8_bwd_kernel(
         for (int e = 0; e < 8; e++) o[e] = rms * (fw[e] * fd[e] - fn[e] * corr);
         if (add_to) {
             float fa[8];
-            unpack8(add_to[at + i], fa);
+            unpack8(a[j], fa);
 #pragma unroll
             for (int e = 0; e < 8; e++) o[e] += fa[e];   // one rounding, at the store
         }
@@ -447,18 +462,20 @@ int ta_silu_mul_q8_bwd(ta_ctx* ctx, const void* dout, const void* gate_q, const 
     });
 }
 
-// Threads a row and vectors a thread by the row's length: a warp up to 1024 columns, else the CTA whose threads hold 4 or 8
-// vectors each.
-#define TA_NORM_CASES(LAUNCH)                                  \
+// Threads a row and vectors a thread by the row's length, each the fastest of those measured on 16384 rows (us, forward / backward
+// at the longest row of the class; in parentheses the next best): 64 x 2 at 1024 columns 26.9 / 22.7 (a warp 28.3 / 25.0), 128 x 2
+// at 2048 49.4 / 39.6 (64 x 4 49.8 / 42.3), 128 x 4 at 3584 83.6 / 67.3 (256 x 2 82.8 / 70.1), at 8192 forward 256 x 4 183 (128 x 8
+// 185) and backward, which holds three arrays, 128 x 8 154 (256 x 4 168).
+#define TA_NORM_CASES(LAUNCH, AT_8192, AT_16384)               \
     do {                                                       \
         const int nvec = D / 8;                                \
         if (nvec <= 32)        LAUNCH(32, 1);                  \
         else if (nvec <= 64)   LAUNCH(32, 2);                  \
-        else if (nvec <= 128)  LAUNCH(32, 4);                  \
+        else if (nvec <= 128)  LAUNCH(64, 2);                  \
         else if (nvec <= 256)  LAUNCH(128, 2);                 \
         else if (nvec <= 512)  LAUNCH(128, 4);                 \
-        else if (nvec <= 1024) LAUNCH(256, 4);                 \
-        else                   LAUNCH(256, 8);                 \
+        else if (nvec <= 1024) LAUNCH AT_8192;                 \
+        else                   LAUNCH AT_16384;                \
     } while (0)
 
 int ta_add_rms_norm_q8_fwd(ta_ctx* ctx, const void* x, const void* delta, const void* w, void* res_out, void* out, void* q, void* scale,
@@ -475,7 +492,7 @@ int ta_add_rms_norm_q8_fwd(ta_ctx* ctx, const void* x, const void* delta, const 
     const auto S = static_cast<uint8_t*>(scale);
 #define TA_LAUNCH(TPR, NV) \
     add_rms_norm_q8_fwd_kernel<TPR, NV><<<TPR == 32 ? (rows + 3) / 4 : rows, TPR == 32 ? 128 : TPR, 0, s>>>(X, De, W, R, O, Q, S, rms_out, rows, D, eps)
-    TA_NORM_CASES(TA_LAUNCH);
+    TA_NORM_CASES(TA_LAUNCH, (256, 4), (256, 8));
 #undef TA_LAUNCH
     TA_LAUNCH_CHECK(ctx, "add_rms_norm_q8_fwd_kernel");
     return TA_OK;
@@ -493,7 +510,7 @@ int ta_rms_norm_q8_bwd(ta_ctx* ctx, const void* dy, const void* q, const void* s
     const auto DX = static_cast<uint4*>(dx);
 #define TA_LAUNCH(TPR, NV) \
     rms_norm_q8_bwd_kernel<TPR, NV><<<TPR == 32 ? (rows + 3) / 4 : rows, TPR == 32 ? 128 : TPR, 0, s>>>(DY, Q, S, W, rms_saved, DX, AT, rows, D)
-    TA_NORM_CASES(TA_LAUNCH);
+    TA_NORM_CASES(TA_LAUNCH, (128, 8), (512, 4));
 #undef TA_LAUNCH
     TA_LAUNCH_CHECK(ctx, "rms_norm_q8_bwd_kernel");
     return TA_OK;
