@@ -195,5 +195,7 @@ def ptr(t) -> c_void_p:
 
 
 def stream_ptr() -> c_void_p:
+    """torch's current stream on the current device.  Its raw handle is asked for directly: building the Stream object that
+    torch.cuda.current_stream() returns takes 3.4 us, as long as a small kernel."""
     import torch
-    return c_void_p(torch.cuda.current_stream().cuda_stream)
+    return c_void_p(torch._C._cuda_getCurrentRawStream(torch.cuda.current_device()))
