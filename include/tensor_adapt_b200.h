@@ -230,7 +230,7 @@ int ta_silu_mul_q8_bwd(ta_ctx* ctx, const void* dout, const void* gate_q, const 
  *     C[M,N] (+)= alpha * col[n] * sum_k A[k][m] * value[k][n]
  * A [K][lda] BF16 (dh, of one adapter or of several that share the input), q / scale [K][N] as above, col [N] BF16 or NULL,
  * C FP32 row-major with pitch ldc, added to if accumulate != 0.  M, N and lda multiples of 8; K may be 0.  Sums in FP32, in an
- * order that depends on M, N and K alone: the same bits every time. */
+ * order that depends on M, N, K and the device alone: the same bits every time. */
 int ta_gemm_tokens_q8_f32(ta_ctx* ctx, int M, int N, int K, float alpha, const void* A, long lda, const void* q, const void* scale,
                           const void* col, float* C, long ldc, int accumulate, void* stream);
 

@@ -6,16 +6,24 @@
 // tokens, the slow axis of both operands, and the scale changes along it, so it cannot be taken out of the sum.
 //
 // A CTA takes 128 columns of q and a share of the tokens, 128 at a time (a chunk).  q, its scales and the matching rows of A come
-// into shared memory asynchronously, chunks ahead.  Warps widen q to BF16 with its scale (exact), pairing tokens on the way, and
-// store it to tensor memory as the K-major first operand [128 columns][tokens] of tcgen05.mma; A is the second, MN-major, from
-// shared memory; D [128 columns][M ranks] is in tensor memory too.  tcgen05.mma cuts its sums off instead of rounding them (8e-6 of
-// the result after 512 products in a row, 1.4e-6 after 128), so after every four chunks, 32 products, D is added to a running sum
-// beside it, rounded, and starts again.  The CTAs on the same columns are a cluster, which adds its
-// sums through distributed shared memory in a fixed order: no partial sums in global memory, no second launch, the same bits
-// every time.
+// into shared memory asynchronously.  Warps widen q to BF16 with its scale (exact), pairing tokens on the way, and store it to
+// tensor memory as the K-major first operand [128 columns][tokens] of tcgen05.mma; A is the second, MN-major, from shared memory;
+// D [128 columns][M ranks] is in tensor memory too.  The CTAs on the same columns are a cluster, which adds its sums through
+// distributed shared memory in a fixed order: no partial sums in global memory, no second launch, the same bits every time.
+//
+// tcgen05.mma cuts its sums off instead of rounding them: 8e-6 of the result after 512 products in a row, 1.4e-6 after 128.  So
+// after every four chunks, 32 products, D is added to a running sum beside it, rounded, and starts again (3e-7 in all).
+//
+// What bounds it is the instructions of the widening (issue 70 % busy with two CTAs an SM), 0.9 us a chunk on each of the two, and
+// 8 us whatever the size: launch, first loads, join.  Measured (us; the bytes at the copy rate in parentheses): 16384 tokens x 18944
+// columns, rank 16, 79 (49); 8192 x 8960, rank 64, 27 (12); 8192 x 896, rank 48, 14 (1.3); 8192 x 3584, rank 192, 25 (5).  Other
+// arrangements at the first: mma.sync from registers 66 and at the second 50, where its products alone take 17; the widened
+// operand in shared memory instead, 97 (6 bytes of its traffic an element); q straight to the widening warps' registers, 94 (the
+// proxy fence after a chunk waits for the loads in flight).
 #include <cooperative_groups.h>
 
 #include <algorithm>
+#include <climits>
 
 #include "act8.cuh"
 #include "ctx.h"
@@ -26,21 +34,23 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kFeat = 128, kTok = 128;      // a chunk: columns of q, tokens
-constexpr int kConv = 8;                    // warps that widen q; then some that bring in q and scales, one for A, one that issues the products
+constexpr int kConv = 8;                    // warps that widen q, in two sets; behind them loaders of q, one of A, one that multiplies
 constexpr int kPitch = kFeat + 4;           // of the sums in shared memory
 
 constexpr int kRun = 4;                     // chunks that D takes in a row
 
-// NB: room for ranks, 64, 128 or 192.  Rings: RS chunks of q and scales, BS of A's rows, two of the widened operand.
+// NB: room for ranks, 64, 128 or 192.  Rings: RS chunks of q and scales, BS of A's rows, two of the widened operand.  The sets of
+// widening warps and the loaders of the TMA form take chunks in turn.  A wait on a barrier's parity cannot tell phases two apart, so
+// nobody may come to a slot whose phase before last is not complete: with an even ring and two of each, a slot is always the same
+// set's and the same loader's, which has waited for that phase itself.
 // WIDE: rows of q start on 16 bytes (N % 16 == 0) and come by TMA; otherwise on 8, by cp.async, which takes more warps.
 template <int NB, bool WIDE, int RS, int BS>
 struct Tile {
-    // The loaders of the TMA form take chunks in turn, no more of them than slots: a parity wait cannot tell phases two apart.
     static constexpr int kLoad = WIDE ? 2 : 6, kThreads = 32 * (kConv + kLoad + 2);
-    static_assert(!WIDE || kLoad <= RS, "");
+    static_assert(RS % 2 == 0, "");
     static constexpr int kBoxes = NB / 64;                          // of A, 64 ranks (128 bytes) wide
     static constexpr int kQ = kFeat * kTok, kBox = kTok * 128, kB = kBoxes * kBox;
-    static constexpr int kScale = kTok * (kFeat / kQ8Block);
+    static constexpr int kScale = kTok * (kFeat / kQ8Block) * 2;     // as BF16
     static constexpr int kAtB = RS * kQ, kAtS = kAtB + BS * kB;
     static constexpr int kRings = kAtS + RS * kScale, kRed = NB * kPitch * 4;
     static constexpr int kSmem = (kRings > kRed ? kRings : kRed) + 1024;
@@ -59,10 +69,16 @@ __device__ __forceinline__ float2 widen2(uint32_t w, int high) {
     asm("cvt.rn.f16x2.e4m3x2 %0, %1;" : "=r"(h) : "h"(uint16_t(high ? w >> 16 : w)));
     return __half22float2(*reinterpret_cast<const __half2*>(&h));
 }
-// Registers of two 16 x 8 mma fragments of 32-bit values (lane / 4 the row, lane % 4 the column, rows 8 on in the odd registers) to
-// 16 lanes and 8 columns of tensor memory.
-__device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&r)[4]) {
-    asm volatile("tcgen05.st.sync.aligned.16x128b.x2.b32 [%0], {%1, %2, %3, %4};" ::"r"(taddr), "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]) : "memory");
+// Registers of 16 x 4 fragments of 32-bit values side by side (lane / 4 the row, lane % 4 the column, rows 8 on in the odd registers) to
+// 16 lanes and 16 columns of tensor memory.
+__device__ __forceinline__ void tmem_st_frag(uint32_t taddr, const uint32_t (&r)[8]) {
+    asm volatile("tcgen05.st.sync.aligned.16x128b.x4.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"r"(taddr), "r"(r[0]), "r"(r[1]),
+                 "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]) : "memory");
+}
+__device__ __forceinline__ uint2 lds64(uint32_t at) {
+    uint2 v;
+    asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "r"(at) : "memory");
+    return v;
 }
 __device__ __forceinline__ uint32_t lds32(uint32_t at) {
     uint32_t v;
@@ -101,10 +117,10 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
         prefetch_tensormap(&a_map);
         for (int i = 0; i < RS; i++) {
             mbar_init(&q_full[i], WIDE ? 2 : 1 + 32 * kLoad);
-            mbar_init(&q_empty[i], kConv);
+            mbar_init(&q_empty[i], kConv / 2);
         }
         for (int i = 0; i < 2; i++) {
-            mbar_init(&x_full[i], kConv);
+            mbar_init(&x_full[i], kConv / 2);
             mbar_init(&x_empty[i], 1);
         }
         for (int i = 0; i < BS; i++) {
@@ -112,7 +128,7 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
             mbar_init(&b_empty[i], 1);
         }
         mbar_init(&d_full, 1);
-        mbar_init(&d_empty, kConv);
+        mbar_init(&d_empty, kConv / 2);
         mbar_init(&done, 1);
         abort_word = 0;
         fence_barrier_init();
@@ -132,36 +148,46 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
     // as one: none may arrive on a barrier once more than its phase expects.
     auto warp_wait = [&](uint64_t* bar, uint32_t parity, int code) { return __all_sync(0xffffffffu, mbar_wait(bar, parity, abort_flag, status, code)) != 0; };
     if (warp < kConv) {
-        // A warp has the 32 lanes of tensor memory, that is the block of 32 columns, that its number allows, and half of the tokens.
-        // Of each step of 16 tokens a thread reads four columns of tokens 2t, 2t + 1, 2t + 8 and 2t + 9 (t: lane % 4, g: lane / 4):
-        // columns 4g and 4g + 1 become rows g and g + 8 of a fragment, 4g + 2 and 4g + 3 those of a second one.  128-byte rows are
-        // swizzled, chunk of 16 bytes c of row r at c ^ (r & 7): the four rows of a load fall on different banks.
-        const int g = lane >> 2, t = lane & 3, blk = warp & 3, tok = (warp >> 2) * (kTok / 2);
-        const uint32_t even = (tok + 2 * t) * 128 + (((blk * 2 + (g >> 2)) ^ (2 * t)) * 16 | (g * 4 & 15)), odd = (even + 128) ^ 16;
-        const uint32_t s_src = base + T::kAtS + ((tok / 16 * 4 + t) * 4 + blk) * 4;
-        const uint32_t x_dst = x_tmem + tok / 2 + quarter;
-        int rs = 0;
-        uint32_t r_phase = 0;
-        for (int i = 0; i < mine; i++) {
+        // A set of four warps widens every other chunk.  A warp has the 32 lanes of tensor memory, that is the block of 32 columns,
+        // that its number allows.  Of each step of 16 tokens a thread reads four columns of tokens 2t, 2t + 1, 2t + 8 and 2t + 9
+        // (t: lane % 4, g: lane / 4): columns 4g and 4g + 1 become rows g and g + 8 of a fragment, 4g + 2 and 4g + 3 those of a
+        // second one.  128-byte rows are swizzled, chunk of 16 bytes c of row r at c ^ (r & 7): the four rows of a load fall on
+        // different banks.
+        const int g = lane >> 2, t = lane & 3, blk = warp & 3, set = warp >> 2;
+        const uint32_t even = 2 * t * 128 + (((blk * 2 + (g >> 2)) ^ (2 * t)) * 16 | (g * 4 & 15)), odd = (even + 128) ^ 16;
+        const uint32_t s_src = base + T::kAtS + (t * 4 + blk) * 8, x_dst = x_tmem + set * T::kX + quarter;
+        int rs = set;
+        uint32_t r_phase = 0, x_phase = 1;
+        for (int i = set; i < mine; i += 2) {
             if (!warp_wait(&q_full[rs], r_phase, DS_TIMEOUT_MMA)) break;
-            if (!warp_wait(&x_empty[i & 1], (i >> 1 & 1) ^ 1, DS_TIMEOUT_PRODUCER)) break;
+            if (!warp_wait(&x_empty[set], x_phase, DS_TIMEOUT_PRODUCER)) break;
             tcgen05_fence_after_sync();
-            const uint32_t src = base + rs * T::kQ;
+            const uint32_t src = base + rs * T::kQ, ssrc = s_src + rs * T::kScale;
 #pragma unroll
-            for (int k = 0; k < kTok / 32; k++) {
-                uint32_t w[4];
-                w[0] = lds32(src + even + k * 2048);
-                w[1] = lds32(src + odd + k * 2048);
-                w[2] = lds32(src + even + k * 2048 + 1024);
-                w[3] = lds32(src + odd + k * 2048 + 1024);
-                const uint32_t s = lds32(s_src + rs * T::kScale + k * 64);
-                const uint32_t s0 = __byte_perm(s, 0, 0x4140) << 7, s1 = __byte_perm(s, 0, 0x4342) << 7;   // BF16's 2^k, two tokens
+            for (int k = 0; k < kTok / 32; k++) {      // two steps
+                uint32_t w[2][4];
+                uint2 s[2];
+#pragma unroll
+                for (int u = 0; u < 2; u++) {
+                    const uint32_t at = src + (2 * k + u) * 2048;
+                    w[u][0] = lds32(at + even);
+                    w[u][1] = lds32(at + odd);
+                    w[u][2] = lds32(at + even + 1024);
+                    w[u][3] = lds32(at + odd + 1024);
+                    s[u] = lds64(ssrc + (2 * k + u) * 128);
+                }
 #pragma unroll
                 for (int h = 0; h < 2; h++) {
-                    const float2 v0 = widen2(w[0], h), v1 = widen2(w[1], h), v2 = widen2(w[2], h), v3 = widen2(w[3], h);
-                    const uint32_t x[4] = {mul_bf16x2(pack_bf16x2(v0.x, v1.x), s0), mul_bf16x2(pack_bf16x2(v0.y, v1.y), s0),
-                                           mul_bf16x2(pack_bf16x2(v2.x, v3.x), s1), mul_bf16x2(pack_bf16x2(v2.y, v3.y), s1)};
-                    tmem_st_frag(x_dst + (i & 1) * T::kX + k * 8 + (uint32_t(h * 16) << 16), x);
+                    uint32_t x[8];
+#pragma unroll
+                    for (int u = 0; u < 2; u++) {
+                        const float2 v0 = widen2(w[u][0], h), v1 = widen2(w[u][1], h), v2 = widen2(w[u][2], h), v3 = widen2(w[u][3], h);
+                        x[4 * u] = mul_bf16x2(pack_bf16x2(v0.x, v1.x), s[u].x);
+                        x[4 * u + 1] = mul_bf16x2(pack_bf16x2(v0.y, v1.y), s[u].x);
+                        x[4 * u + 2] = mul_bf16x2(pack_bf16x2(v2.x, v3.x), s[u].y);
+                        x[4 * u + 3] = mul_bf16x2(pack_bf16x2(v2.y, v3.y), s[u].y);
+                    }
+                    tmem_st_frag(x_dst + k * 16 + (uint32_t(h * 16) << 16), x);
                 }
             }
             __syncwarp();
@@ -169,11 +195,11 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
             tmem_st_wait();
             tcgen05_fence_before_sync();
             __syncwarp();
-            if (lane == 0) mbar_arrive(&x_full[i & 1]);
+            if (lane == 0) mbar_arrive(&x_full[set]);
             if (i > 0 && i % kRun == 0) {      // the run before this chunk
                 if (!warp_wait(&d_full, (i / kRun - 1) & 1, DS_TIMEOUT_EPILOGUE)) break;
                 tcgen05_fence_after_sync();
-                for (int n = (warp >> 2) * 16; n < ranks; n += 32) {
+                for (int n = 0; n < ranks; n += 16) {
                     uint32_t d[16], old[16];
                     tmem_ld_x16(d_tmem + n + quarter, d);
                     if (i > kRun) tmem_ld_x16(s_tmem + n + quarter, old);
@@ -192,18 +218,19 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
                 __syncwarp();
                 if (lane == 0) mbar_arrive(&d_empty);
             }
-            if (++rs == RS) { rs = 0; r_phase ^= 1; }
+            if ((rs += 2) >= RS) { rs -= RS; r_phase ^= 1; }
+            x_phase ^= 1;
         }
     } else if (warp < kConv + kLoad) {
         // By TMA the warps take chunks in turn; by cp.async all work on every chunk, and the first has the scales.  Those are too
         // small and unaligned for an asynchronous copy: a lane reads the four blocks' bytes of tokens 2t, 2t + 1, 2t + 8 and 2t + 9
-        // of a step of 16 (t: lane % 4, the step: lane / 4), AHEAD of its chunks ahead, and stores a word of four tokens for each.
-        constexpr int AHEAD = 2;
+        // of a step of 16 (t: lane % 4, the step: lane / 4) one chunk ahead, and stores them as BF16 pairs.  (Two ahead is slower by
+        // 1 to 2 us, the lines of L1 that the reads in flight hold are too many.)
         const int nblk = (N + kQ8Block - 1) / kQ8Block, blk0 = f0 / kQ8Block, me = warp - kConv;
         constexpr int kTurn = WIDE ? kLoad : 1;
         const int first = WIDE ? me : 0;
         const bool words = nblk % 4 == 0 && (reinterpret_cast<uintptr_t>(scale) & 3) == 0;    // then so are four blocks of a row
-        uint32_t held[AHEAD][4];
+        uint32_t held[4];
         auto read = [&](int i, uint32_t (&h)[4]) {
             const int tok0 = (i * cs + rank) * kTok + (lane >> 2) * 16 + (lane & 3) * 2;
 #pragma unroll
@@ -242,23 +269,23 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
                 cp_async_arrive(&q_full[rs]);
                 if (me != 0) return true;
             }
-            const uint32_t lo0 = __byte_perm(h[0], h[1], 0x5140), hi0 = __byte_perm(h[0], h[1], 0x7362);
-            const uint32_t lo1 = __byte_perm(h[2], h[3], 0x5140), hi1 = __byte_perm(h[2], h[3], 0x7362);
-            reinterpret_cast<uint4*>(smem + T::kAtS + rs * T::kScale)[lane] =
-                make_uint4(__byte_perm(lo0, lo1, 0x5410), __byte_perm(lo0, lo1, 0x7632), __byte_perm(hi0, hi1, 0x5410), __byte_perm(hi0, hi1, 0x7632));
+            uint32_t pair[8];       // BF16's 2^k of tokens 2t and 2t + 1, and of 2t + 8 and 2t + 9, for each block
+#pragma unroll
+            for (int b = 0; b < 4; b++) {
+                pair[2 * b] = (h[0] >> 8 * b & 0xFF) << 7 | (h[1] >> 8 * b & 0xFF) << 23;
+                pair[2 * b + 1] = (h[2] >> 8 * b & 0xFF) << 7 | (h[3] >> 8 * b & 0xFF) << 23;
+            }
+            uint4* to = reinterpret_cast<uint4*>(smem + T::kAtS + rs * T::kScale) + lane * 2;
+            to[0] = make_uint4(pair[0], pair[1], pair[2], pair[3]);
+            to[1] = make_uint4(pair[4], pair[5], pair[6], pair[7]);
             __syncwarp();
             if (lane == 0) mbar_arrive(&q_full[rs]);
             return true;
         };
-#pragma unroll
-        for (int d = 0; d < AHEAD; d++) read(first + d * kTurn, held[d]);
-        bool ok = true;
-        for (int i = first; i < mine && ok; i += AHEAD * kTurn) {
-#pragma unroll
-            for (int d = 0; d < AHEAD; d++) {
-                if (ok && i + d * kTurn < mine) ok = copy(i + d * kTurn, held[d]);
-                read(i + (d + AHEAD) * kTurn, held[d]);
-            }
+        read(first, held);
+        for (int i = first; i < mine; i += kTurn) {
+            if (!copy(i, held)) break;
+            read(i + kTurn, held);
         }
     } else if (warp == kConv + kLoad) {
         if (lane == 0) {
@@ -395,7 +422,7 @@ void ask(F kernel, cudaLaunchConfig_t cfg, cudaLaunchAttribute& at, int per_sm, 
 }
 
 template <int NB, bool WIDE, int RS, int BS>
-int launch(const Call& c, int force_cs = 0) {
+int launch(const Call& c) {
     using T = Tile<NB, WIDE, RS, BS>;
     ta_ctx* ctx = c.ctx;
     const auto kernel = gemm_tokens_q8_kernel<NB, WIDE, RS, BS>;
@@ -424,7 +451,6 @@ int launch(const Call& c, int force_cs = 0) {
         if (cs == 0 || cost < least) { least = cost; cs = 1 << k; }
     }
     if (cs == 0) return fail(ctx, TA_ERR_CUDA, "gemm_tokens_q8_f32: the kernel cannot be resident on this device");
-    if (force_cs) cs = force_cs;
     at.val.clusterDim.x = unsigned(cs);
     cfg.gridDim = dim3(tiles * unsigned(cs), rows);
     CUtensorMap q_map{}, a_map;
@@ -435,9 +461,11 @@ int launch(const Call& c, int force_cs = 0) {
     TA_LAUNCH_CHECK(ctx, "gemm_tokens_q8_kernel");
     return TA_OK;
 }
+// Rings: with NB 64, 67 KB a CTA leave L1 to the scale reads (four slots of q instead of two: 81 -> 79 us at rank 16, 27 -> 28.5 at
+// rank 64); the larger ones have an SM to themselves.  Above 192 ranks, passes of 128.
 template <bool WIDE>
 int launch_for_rank(const Call& c) {
-    return c.M <= 64 ? launch<64, WIDE, 3, 2>(c) : c.M <= 128 ? launch<128, WIDE, 4, 2>(c) : c.M <= 192 ? launch<192, WIDE, 4, 2>(c) : launch<128, WIDE, 4, 2>(c);
+    return c.M <= 64 ? launch<64, WIDE, 2, 2>(c) : c.M <= 128 ? launch<128, WIDE, 4, 2>(c) : c.M <= 192 ? launch<192, WIDE, 4, 2>(c) : launch<128, WIDE, 4, 2>(c);
 }
 
 }  // namespace
@@ -449,6 +477,7 @@ extern "C" int ta_gemm_tokens_q8_f32(ta_ctx* ctx, int M, int N, int K, float alp
                                      const void* col, float* C, long ldc, int accumulate, void* stream) {
     if (!ctx || !A || !q || !scale || !C || M <= 0 || N <= 0 || K < 0)
         return fail(ctx, TA_ERR_INVALID, "gemm_tokens_q8_f32: null argument or bad size");
+    if (K > INT_MAX - 8 * kTok) return fail(ctx, TA_ERR_UNSUPPORTED, "gemm_tokens_q8_f32: more than 2^31 - 1025 tokens");
     if (M % 8 || N % 8 || lda % 8 || lda < M || ldc < N)
         return fail(ctx, TA_ERR_INVALID, "gemm_tokens_q8_f32: M, N and lda must be multiples of 8, lda >= M, ldc >= N");
     if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(q) & 15))
