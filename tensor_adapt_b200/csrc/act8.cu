@@ -200,13 +200,14 @@ __global__ void __launch_bounds__(kThreads) silu_mul_q8_bwd_kernel(Rows r, const
 // 16384 x 3584, a warp a row 100).  All loads of a row stand before its sum, add_to's too (after it: 77 us).
 //
 // Sum over the threads of a row; every thread gets it.  A warp's sum needs no barrier; a CTA's one.
-template <int TPR>
-__device__ __forceinline__ float row_sum(float v, float* red) {
-    v = warp_sum(v);
+template <int TPR, typename T>
+__device__ __forceinline__ T row_sum(T v, T* red) {
+#pragma unroll
+    for (int o = 16; o > 0; o >>= 1) v += __shfl_xor_sync(0xffffffffu, v, o);
     if constexpr (TPR > 32) {
         if ((threadIdx.x & 31) == 0) red[threadIdx.x >> 5] = v;
         __syncthreads();
-        v = 0.f;
+        v = 0;
 #pragma unroll
         for (int w = 0; w < TPR / 32; w++) v += red[w];
     }
@@ -215,18 +216,22 @@ __device__ __forceinline__ float row_sum(float v, float* red) {
 
 // r = bf16(x + delta), n = r / rms(r), out = bf16(n * w), (q, scale) = n in 8 bits.  n and not n * w is held: the backward
 // needs n, and a gradient over tokens of out = n * w has w as a factor of its columns (ta_gemm_tokens_q8_f32's `col`).
+// 1 / rms is formed in 64 bits from sums of eight squares and multiplied as two FP32 parts, the product is cut off and its last bit
+// set, so that its conversion to e4m3 and its comparison with 448 * 2^k come out as the unrounded product's: next to a border an
+// error of 1e-7 gives another code, or to all 32 of a block another scale.  It costs 2 us of 87 at 16384 x 3584 (81 at the
+// copy rate).
 template <int TPR, int NV>
 __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) add_rms_norm_q8_fwd_kernel(const uint4* x, const uint4* delta, const uint4* __restrict__ w,
                                                                                     uint4* res, uint4* out, uint2* q, uint8_t* scale,
-                                                                                    float* rms_out, int rows, int D, float eps) {
-    __shared__ float red[TPR / 32];
+                                                                                    float* rms_out, int rows, int D, double inv_d, float eps) {
+    __shared__ double red[TPR / 32];
     const int lane = threadIdx.x % TPR;
     const int row = TPR == 32 ? blockIdx.x * (blockDim.x / 32) + threadIdx.x / 32 : blockIdx.x;
     if (row >= rows) return;   // a whole warp's, or a whole CTA's
     const int nvec = D / 8, nblk = (D + kQ8Block - 1) / kQ8Block;
     const size_t at = size_t(row) * nvec;
     uint4 v[NV];
-    float ss = 0.f;
+    double ss = 0;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int i = lane + j * TPR;
@@ -259,13 +264,15 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) add_rms_norm_q8_fwd_ker
     }
 #pragma unroll
     for (int j = 0; j < NV; j++) {
-        float f[8];
+        float f[8], eight = 0.f;
         unpack8(v[j], f);
 #pragma unroll
-        for (int e = 0; e < 8; e++) ss += f[e] * f[e];
+        for (int e = 0; e < 8; e++) eight += f[e] * f[e];
+        ss += double(eight);
     }
     ss = row_sum<TPR>(ss, red);
-    const float rms = 1.0f / sqrtf(ss / float(D) + eps);
+    const double exact = rsqrt(ss * inv_d + double(eps));
+    const float rms = float(exact), rest = exact < double(CUDART_INF_F) ? float(exact - double(rms)) : 0.f;
     if (lane == 0) rms_out[row] = rms;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
@@ -273,7 +280,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) add_rms_norm_q8_fwd_ker
         float f[8];
         unpack8(v[j], f);
 #pragma unroll
-        for (int e = 0; e < 8; e++) f[e] *= rms;
+        for (int e = 0; e < 8; e++) f[e] = __uint_as_float(__float_as_uint(__fmaf_rz(f[e], rms, f[e] * rest)) | 1u);
         int byte;
         const uint2 o = narrow8(f, byte);
         if (i < nvec) {
@@ -491,7 +498,7 @@ int ta_add_rms_norm_q8_fwd(ta_ctx* ctx, const void* x, const void* delta, const 
     const auto Q = static_cast<uint2*>(q);
     const auto S = static_cast<uint8_t*>(scale);
 #define TA_LAUNCH(TPR, NV) \
-    add_rms_norm_q8_fwd_kernel<TPR, NV><<<TPR == 32 ? (rows + 3) / 4 : rows, TPR == 32 ? 128 : TPR, 0, s>>>(X, De, W, R, O, Q, S, rms_out, rows, D, eps)
+    add_rms_norm_q8_fwd_kernel<TPR, NV><<<TPR == 32 ? (rows + 3) / 4 : rows, TPR == 32 ? 128 : TPR, 0, s>>>(X, De, W, R, O, Q, S, rms_out, rows, D, 1.0 / D, eps)
     TA_NORM_CASES(TA_LAUNCH, (256, 4), (256, 8));
 #undef TA_LAUNCH
     TA_LAUNCH_CHECK(ctx, "add_rms_norm_q8_fwd_kernel");
