@@ -93,6 +93,7 @@ _PROTOS = {
     "ta_allreduce_grads": (c_int, [P, P]),
     "ta_trainer_set_comm": (c_int, [P, P]),
     "ta_trainer_create": (c_int, [P, P, P, c_int, c_int, P, POINTER(c_void_p)]),
+    "ta_trainer_create_ex": (c_int, [P, P, P, c_int, c_int, c_int, P, POINTER(c_void_p)]),
     "ta_trainer_destroy": (c_int, [P]),
     "ta_trainer_init_random": (c_int, [P, ctypes.c_ulonglong, c_float]),
     "ta_trainer_tensor": (c_int, [P, c_char_p, POINTER(c_void_p), POINTER(c_long), POINTER(c_long), POINTER(c_long),

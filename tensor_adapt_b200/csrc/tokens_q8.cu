@@ -457,6 +457,7 @@ int launch(const Call& c) {
     if (WIDE)
         if (int rc = encode_tmap_2d(ctx, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.q, c.N, c.K, c.N, kFeat, kTok, 128, &q_map)) return rc;
     if (int rc = encode_tmap_2d(ctx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c.A, c.M, c.K, c.lda * 2, 64, kTok, 128, &a_map)) return rc;
+    ProfScope prof(ctx, c.stream, PROF_GEMM_SKINNY, 2.0 * c.M * c.N * c.K);
     TA_CUDA(ctx, cudaLaunchKernelEx(&cfg, kernel, q_map, a_map, c.q, c.scale, c.col, c.C, c.ldc, c.M, c.N, c.K, c.alpha, c.accumulate, ctx->d_status));
     TA_LAUNCH_CHECK(ctx, "gemm_tokens_q8_kernel");
     return TA_OK;

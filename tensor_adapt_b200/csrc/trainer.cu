@@ -153,6 +153,25 @@ int proj_gate_up_swiglu(ta_trainer* t, int l, const bf16* x, int BT) {
 }
 
 struct BwdProj { const bf16* dY; const bf16* W; int tgt; };
+// gA (of one adapter, or of several with contiguous blocks) += dh_s^T.x (tiles [in][r], stored transposed)
+int grad_a(ta_trainer* t, const bf16* x, int in, const bf16* dh, int r, float* gA, int BT) {
+    GemmSegment g; g.A = x; g.lda = in; g.a_mn = true; g.B = dh; g.ldb = r; g.b_mn = true; g.K = BT;
+    GemmOut o; o.C = gA; o.ldc = in; o.f32 = true; o.accumulate = true; o.transpose_out = true;
+    o.split_k = tokens_gemm_splits(t->ctx, in, r, BT); o.split_ws = t->splitk; o.split_ws_bytes = t->splitk_bytes;
+    return seg_gemm(t->ctx, t->stream, in, r, &g, 1, o);
+}
+// The input of a backward group: x in BF16, or a norm's rows in 8 bits with the norm's weight (x = value * col); with neither, gA is
+// left to the caller (dh_s of a single projection is t->dh[0], [BT][r]).
+struct GroupInput {
+    const bf16* x = nullptr;
+    const Held8* held = nullptr;
+    const bf16* col = nullptr;
+};
+int grad_a_any(ta_trainer* t, const GroupInput& in_x, int in, const bf16* dh, int r, float* gA, int BT) {
+    if (in_x.held)
+        return ta_gemm_tokens_q8_f32(t->ctx, r, in, BT, 1.f, dh, r, in_x.held->q, in_x.held->scale, in_x.col, gA, in, 1, t->stream);
+    return in_x.x ? grad_a(t, in_x.x, in, dh, r, gA, BT) : TA_OK;
+}
 // Optional fused SwiGLU backward on the product of a backward group (the down projection's dX = d_act): the epilogue
 // turns d_act into d_gate / d_up with the forward's gate / up and d_act itself is never stored.
 struct SwigluBwd { const bf16* gate = nullptr; const bf16* up = nullptr; bf16* d_gate = nullptr; bf16* d_up = nullptr; };
@@ -160,7 +179,7 @@ struct SwigluBwd { const bf16* gate = nullptr; const bf16* up = nullptr; bf16* d
 // dX = sum_i dY_i.W_i + sum_i dh_i.A_i in ONE segmented GEMM; gA_i, gB_i accumulated on the way.
 // `fused`: the projections share x and form a fused group (contiguous A / gA blocks, dh slices of one
 // [BT][np*r] buffer), so gA of the whole group is one pass over x.
-int proj_bwd_group(ta_trainer* t, int l, const bf16* x, const BwdProj* ps, int np, bf16* dX, int BT, bool fused,
+int proj_bwd_group(ta_trainer* t, int l, const GroupInput& x, const BwdProj* ps, int np, bf16* dX, int BT, bool fused,
                    const SwigluBwd* swiglu = nullptr) {
     GemmSegment seg[kMaxSegments];
     int nseg = 0, in = 0;
@@ -191,22 +210,12 @@ int proj_bwd_group(ta_trainer* t, int l, const bf16* x, const BwdProj* ps, int n
             o.split_k = tokens_gemm_splits(t->ctx, out, lr.r, BT); o.split_ws = t->splitk; o.split_ws_bytes = t->splitk_bytes;
             RC(seg_gemm(t->ctx, t->stream, out, lr.r, &g, 1, o));
         }
-        if (!fused) {   // gA += dh_s^T.x (tiles [in][r], stored transposed)
-            GemmSegment g; g.A = x; g.lda = in; g.a_mn = true; g.B = dh; g.ldb = dh_ld; g.b_mn = true; g.K = BT;
-            GemmOut o; o.C = lr.gA; o.ldc = in; o.f32 = true; o.accumulate = true; o.transpose_out = true;
-            o.split_k = tokens_gemm_splits(t->ctx, in, lr.r, BT); o.split_ws = t->splitk; o.split_ws_bytes = t->splitk_bytes;
-            RC(seg_gemm(t->ctx, t->stream, in, lr.r, &g, 1, o));
-        }
+        if (!fused) RC(grad_a_any(t, x, in, dh, lr.r, lr.gA, BT));
         GemmSegment& g = seg[nseg++];
         g.A = dh; g.lda = dh_ld; g.B = lr.A; g.ldb = in; g.b_mn = true; g.K = lr.r;
     }
-    if (fused) {   // gA of the whole group: [in][np*r] tiles stored transposed into the contiguous gA blocks
-        LoraRef first = t->ref(l, ps[0].tgt);
-        GemmSegment g; g.A = x; g.lda = in; g.a_mn = true; g.B = t->dh[0]; g.ldb = np * r; g.b_mn = true; g.K = BT;
-        GemmOut o; o.C = first.gA; o.ldc = in; o.f32 = true; o.accumulate = true; o.transpose_out = true;
-        o.split_k = tokens_gemm_splits(t->ctx, in, np * r, BT); o.split_ws = t->splitk; o.split_ws_bytes = t->splitk_bytes;
-        RC(seg_gemm(t->ctx, t->stream, in, np * r, &g, 1, o));
-    }
+    // gA of the whole group: [in][np*r] tiles stored transposed into the contiguous gA blocks
+    if (fused) RC(grad_a_any(t, x, in, t->dh[0], np * r, t->ref(l, ps[0].tgt).gA, BT));
     GemmOut o;
     o.C = dX; o.ldc = in;
     if (swiglu) { o.epi = 2; o.C = swiglu->d_gate; o.C2 = swiglu->d_up; o.gate_in = swiglu->gate; o.up_in = swiglu->up; }
@@ -223,7 +232,8 @@ int run_micro(ta_trainer* t, int Bm, int T, float inv_count, bool exchange) {
     const int BT = Bm * T, H = c.hidden, I = c.intermediate, qd = c.q_heads * c.head_dim, kv = c.kv_heads * c.head_dim;
     const int Lyr = c.layers;
     // SwiGLU folded into the GEMM epilogues (no act / d_act round trips) whenever the 256-row tile kernels apply
-    const bool swiglu_fused = t->fuse_swiglu < 0 ? seg_gemm_swiglu_pays(ctx, BT) : (t->fuse_swiglu != 0 && seg_gemm_supports_swiglu(ctx, BT));
+    // (with 8-bit activations the separate SwiGLU kernels, which leave and read gate and up in 8 bits)
+    const bool swiglu_fused = t->act8 ? false : t->fuse_swiglu < 0 ? seg_gemm_swiglu_pays(ctx, BT) : (t->fuse_swiglu != 0 && seg_gemm_supports_swiglu(ctx, BT));
 
     // ── forward ────────────────────────────────────────────────────────────
     RC(ta_embed_fwd(ctx, t->embed, t->tok, t->cache[0].r_in, BT, H, s));
@@ -231,7 +241,10 @@ int run_micro(ta_trainer* t, int Bm, int T, float inv_count, bool exchange) {
         LayerW& w = t->L[l];
         LayerCache& k = t->cache[l];
         bf16* r_next = (l + 1 < Lyr) ? t->cache[l + 1].r_in : t->r_final;
-        RC(ta_rms_norm_fwd(ctx, k.r_in, w.input_norm, k.x_normed, k.in_rms, BT, H, c.rms_eps, s));
+        if (t->act8)
+            RC(ta_add_rms_norm_q8_fwd(ctx, k.r_in, nullptr, w.input_norm, nullptr, k.x_normed, k.norm1.q, k.norm1.scale, k.in_rms, BT, H, c.rms_eps, s));
+        else
+            RC(ta_rms_norm_fwd(ctx, k.r_in, w.input_norm, k.x_normed, k.in_rms, BT, H, c.rms_eps, s));
         if (t->fuse_qkv) RC(lora_down_group(t, l, T_Q, 3, k.x_normed, BT));
         RC(proj_fwd(t, l, T_Q, k.x_normed, w.q_w, w.q_b, nullptr, k.Q, BT, t->fuse_qkv));
         RC(proj_fwd(t, l, T_K, k.x_normed, w.k_w, w.k_b, nullptr, k.K, BT, t->fuse_qkv));
@@ -239,14 +252,18 @@ int run_micro(ta_trainer* t, int Bm, int T, float inv_count, bool exchange) {
         RC(ta_rope(ctx, k.Q, c.q_heads, k.K, c.kv_heads, Bm, T, c.head_dim, c.rope_theta, 0, s));
         RC(ta_flash_attn_fwd(ctx, k.Q, k.K, k.V, k.attn_out, k.lse, Bm, T, c.q_heads, c.kv_heads, c.head_dim, s));
         RC(proj_fwd(t, l, T_O, k.attn_out, w.o_w, nullptr, k.r_in, k.r_mid, BT));          // + residual
-        RC(ta_rms_norm_fwd(ctx, k.r_mid, w.post_norm, k.x_normed2, k.post_rms, BT, H, c.rms_eps, s));
+        if (t->act8)
+            RC(ta_add_rms_norm_q8_fwd(ctx, k.r_mid, nullptr, w.post_norm, nullptr, k.x_normed2, k.norm2.q, k.norm2.scale, k.post_rms, BT, H, c.rms_eps, s));
+        else
+            RC(ta_rms_norm_fwd(ctx, k.r_mid, w.post_norm, k.x_normed2, k.post_rms, BT, H, c.rms_eps, s));
         if (t->fuse_gu) RC(lora_down_group(t, l, T_GATE, 2, k.x_normed2, BT));
         if (swiglu_fused && (t->fuse_gu || (!t->ref(l, T_GATE).on() && !t->ref(l, T_UP).on()))) {
             RC(proj_gate_up_swiglu(t, l, k.x_normed2, BT));
         } else {
             RC(proj_fwd(t, l, T_GATE, k.x_normed2, w.gate_w, nullptr, nullptr, k.gate, BT, t->fuse_gu));
             RC(proj_fwd(t, l, T_UP, k.x_normed2, w.up_w, nullptr, nullptr, k.up, BT, t->fuse_gu));
-            RC(ta_silu_mul_fwd(ctx, k.gate, k.up, k.act, long(BT) * I, s));
+            if (t->act8) RC(ta_silu_mul_q8_fwd(ctx, k.gate, k.up, k.act, k.gate8.q, k.gate8.scale, k.up8.q, k.up8.scale, BT, I, s));
+            else RC(ta_silu_mul_fwd(ctx, k.gate, k.up, k.act, long(BT) * I, s));
         }
         RC(proj_fwd(t, l, T_DOWN, k.act, w.down_w, nullptr, k.r_mid, r_next, BT));         // + residual
     }
@@ -267,32 +284,41 @@ int run_micro(ta_trainer* t, int Bm, int T, float inv_count, bool exchange) {
         LayerCache& k = t->cache[l];
         {   // FFN: dact = grad.Wd (+LoRA down), then dgate / dup                (qwen2.cu:221-230)
             BwdProj p{t->g_res, w.down_w, T_DOWN};
-            if (swiglu_fused) {
+            if (t->act8) {   // act comes back with d_gate / d_up, so gA of down follows them
+                RC(proj_bwd_group(t, l, {}, &p, 1, t->d_act, BT, false));
+                RC(ta_silu_mul_q8_bwd(ctx, t->d_act, k.gate8.q, k.gate8.scale, k.up8.q, k.up8.scale, t->d_gate, t->d_up, k.act, BT, I, s));
+                LoraRef lr = t->ref(l, T_DOWN);
+                if (lr.on()) RC(grad_a(t, k.act, I, t->dh[0], lr.r, lr.gA, BT));
+            } else if (swiglu_fused) {
                 SwigluBwd sw; sw.gate = k.gate; sw.up = k.up; sw.d_gate = t->d_gate; sw.d_up = t->d_up;
-                RC(proj_bwd_group(t, l, k.act, &p, 1, nullptr, BT, false, &sw));
+                RC(proj_bwd_group(t, l, {k.act}, &p, 1, nullptr, BT, false, &sw));
             } else {
-                RC(proj_bwd_group(t, l, k.act, &p, 1, t->d_act, BT, false));
+                RC(proj_bwd_group(t, l, {k.act}, &p, 1, t->d_act, BT, false));
                 RC(ta_silu_mul_bwd(ctx, t->d_act, k.gate, k.up, t->d_gate, t->d_up, long(BT) * I, s));
             }
         }
         {   // dx_normed2 = dgate.Wg + dup.Wu (+LoRA)                           (:232-234)
             BwdProj p[2] = {{t->d_gate, w.gate_w, T_GATE}, {t->d_up, w.up_w, T_UP}};
-            RC(proj_bwd_group(t, l, k.x_normed2, p, 2, t->d_xn, BT, t->fuse_gu));
+            RC(proj_bwd_group(t, l, t->act8 ? GroupInput{nullptr, &k.norm2, w.post_norm} : GroupInput{k.x_normed2}, p, 2, t->d_xn, BT, t->fuse_gu));
         }
         // grad += rms_norm_bwd(dx_normed2, pre_ffn_res)                       (:238-246)
-        RC(ta_rms_norm_bwd(ctx, t->d_xn, k.r_mid, w.post_norm, k.post_rms, t->g_res, t->g_res, BT, H, s));
+        if (t->act8)
+            RC(ta_rms_norm_q8_bwd(ctx, t->d_xn, k.norm2.q, k.norm2.scale, w.post_norm, k.post_rms, t->g_res, t->g_res, BT, H, s));
+        else
+            RC(ta_rms_norm_bwd(ctx, t->d_xn, k.r_mid, w.post_norm, k.post_rms, t->g_res, t->g_res, BT, H, s));
         {   // dx_attn_out = grad.Wo (+LoRA o)                                 (:253-264)
             BwdProj p{t->g_res, w.o_w, T_O};
-            RC(proj_bwd_group(t, l, k.attn_out, &p, 1, t->d_attn, BT, false));
+            RC(proj_bwd_group(t, l, {k.attn_out}, &p, 1, t->d_attn, BT, false));
         }
         RC(ta_flash_attn_bwd(ctx, t->d_attn, k.Q, k.K, k.V, k.attn_out, k.lse, t->dQ, t->dK, t->dV, t->delta, Bm, T,
                              c.q_heads, c.kv_heads, c.head_dim, s));
         RC(ta_rope(ctx, t->dQ, c.q_heads, t->dK, c.kv_heads, Bm, T, c.head_dim, c.rope_theta, 1, s));
         {   // dx_normed = dQ.Wq + dK.Wk + dV.Wv (+LoRA q,k,v)                  (:282-292)
             BwdProj p[3] = {{t->dQ, w.q_w, T_Q}, {t->dK, w.k_w, T_K}, {t->dV, w.v_w, T_V}};
-            RC(proj_bwd_group(t, l, k.x_normed, p, 3, t->d_xn, BT, t->fuse_qkv));
+            RC(proj_bwd_group(t, l, t->act8 ? GroupInput{nullptr, &k.norm1, w.input_norm} : GroupInput{k.x_normed}, p, 3, t->d_xn, BT, t->fuse_qkv));
         }
         // centroid side-channel: hidden = x_normed, signal = dx_normed        (adapt_trainer.cu:210-232)
+        if (t->act8 && (t->ac.centroid_modes & 7)) RC(ta_q8_load(ctx, k.norm1.q, k.norm1.scale, w.input_norm, k.x_normed, BT, H, s));
         if (t->ac.centroid_modes & 1)
             RC(ta_centroid_accumulate(ctx, TA_CENTROID_INTENDED, k.x_normed, t->d_xn, BT, H, t->cen_acc, t->cen_w, s));
         if (t->ac.centroid_modes & 2)
@@ -301,7 +327,9 @@ int run_micro(ta_trainer* t, int Bm, int T, float inv_count, bool exchange) {
             RC(ta_centroid_accumulate(ctx, TA_CENTROID_INTENDED, k.x_normed, t->d_xn, BT, H, t->cen_bank + size_t(l) * H,
                                       t->cen_bank_w + l, s));
         // grad += rms_norm_bwd(dx_normed, pre_attn_res)                       (:298-304)
-        if (l > 0)
+        if (l > 0 && t->act8)
+            RC(ta_rms_norm_q8_bwd(ctx, t->d_xn, k.norm1.q, k.norm1.scale, w.input_norm, k.in_rms, t->g_res, t->g_res, BT, H, s));
+        else if (l > 0)
             RC(ta_rms_norm_bwd(ctx, t->d_xn, k.r_in, w.input_norm, k.in_rms, t->g_res, t->g_res, BT, H, s));
         if (exchange) RC(comm_reduce_slice(t, t->layer_begin[size_t(l)], t->layer_begin[size_t(l) + 1]));
     }
@@ -321,6 +349,11 @@ extern "C" {
 
 int ta_trainer_create(ta_ctx* ctx, const ta_model_config* mc, const ta_adapter_config* ac, int micro_batch, int seq_len,
                       void* stream, ta_trainer** out) {
+    return ta_trainer_create_ex(ctx, mc, ac, micro_batch, seq_len, 16, stream, out);
+}
+
+int ta_trainer_create_ex(ta_ctx* ctx, const ta_model_config* mc, const ta_adapter_config* ac, int micro_batch, int seq_len,
+                         int act_bits, void* stream, ta_trainer** out) {
     if (!ctx || !mc || !ac || !out || micro_batch <= 0 || seq_len <= 0)
         return fail(ctx, TA_ERR_INVALID, "trainer_create: null argument or bad size");
     *out = nullptr;
@@ -331,12 +364,14 @@ int ta_trainer_create(ta_ctx* ctx, const ta_model_config* mc, const ta_adapter_c
     if (c.head_dim != 64 && c.head_dim != 128) return fail(ctx, TA_ERR_UNSUPPORTED, "trainer_create: head_dim 64 or 128");
     if (c.hidden % 8 || c.intermediate % 8 || c.vocab % 8) return fail(ctx, TA_ERR_UNSUPPORTED, "trainer_create: dims % 8");
     if (ac->rank <= 0 || ac->rank > 256) return fail(ctx, TA_ERR_INVALID, "trainer_create: rank must be in 1..256");
+    if (act_bits != 8 && act_bits != 16) return fail(ctx, TA_ERR_INVALID, "trainer_create: act_bits must be 8 or 16");
 
     ta_trainer* t = new ta_trainer();
     t->ctx = ctx; t->stream = static_cast<cudaStream_t>(stream); t->mc = c; t->ac = *ac;
     t->r_pad = (ac->rank + 15) / 16 * 16;
     t->scale = ac->alpha / float(ac->rank);
     t->micro_B = micro_batch; t->T = seq_len;
+    t->act8 = act_bits == 8;
     const long H = c.hidden, I = c.intermediate, V = c.vocab, qd = long(c.q_heads) * c.head_dim,
                kv = long(c.kv_heads) * c.head_dim, BT = long(micro_batch) * seq_len;
     const int Lyr = c.layers, r = t->r_pad;
@@ -415,19 +450,34 @@ int ta_trainer_create(ta_ctx* ctx, const ta_model_config* mc, const ta_adapter_c
         t->stats = t->cen_w + 8;
         // activations
         t->cache.resize(Lyr);
+        auto held8 = [&](long cols) {
+            Held8 h;
+            h.q = static_cast<uint8_t*>(A.take(size_t(BT) * cols));
+            h.scale = static_cast<uint8_t*>(A.take(size_t(BT) * ((cols + TA_Q8_BLOCK - 1) / TA_Q8_BLOCK)));
+            return h;
+        };
         for (int l = 0; l < Lyr; l++) {
             LayerCache& k = t->cache[l];
-            k.r_in = static_cast<bf16*>(A.take(bytes_bf16(BT * H)));
-            k.x_normed = static_cast<bf16*>(A.take(bytes_bf16(BT * H)));
+            if (t->act8 && l > 0) {   // the first layer's buffers serve all
+                const LayerCache& f = t->cache[0];
+                k.r_in = f.r_in; k.x_normed = f.x_normed; k.r_mid = f.r_mid; k.x_normed2 = f.x_normed2;
+                k.gate = f.gate; k.up = f.up; k.act = f.act;
+            } else {
+                k.r_in = static_cast<bf16*>(A.take(bytes_bf16(BT * H)));
+                k.x_normed = static_cast<bf16*>(A.take(bytes_bf16(BT * H)));
+            }
             k.Q = static_cast<bf16*>(A.take(bytes_bf16(BT * qd)));
             k.K = static_cast<bf16*>(A.take(bytes_bf16(BT * kv)));
             k.V = static_cast<bf16*>(A.take(bytes_bf16(BT * kv)));
             k.attn_out = static_cast<bf16*>(A.take(bytes_bf16(BT * qd)));
-            k.r_mid = static_cast<bf16*>(A.take(bytes_bf16(BT * H)));
-            k.x_normed2 = static_cast<bf16*>(A.take(bytes_bf16(BT * H)));
-            k.gate = static_cast<bf16*>(A.take(bytes_bf16(BT * I)));
-            k.up = static_cast<bf16*>(A.take(bytes_bf16(BT * I)));
-            k.act = static_cast<bf16*>(A.take(bytes_bf16(BT * I)));
+            if (!t->act8 || l == 0) {
+                k.r_mid = static_cast<bf16*>(A.take(bytes_bf16(BT * H)));
+                k.x_normed2 = t->act8 ? k.x_normed : static_cast<bf16*>(A.take(bytes_bf16(BT * H)));
+                k.gate = static_cast<bf16*>(A.take(bytes_bf16(BT * I)));
+                k.up = static_cast<bf16*>(A.take(bytes_bf16(BT * I)));
+                k.act = static_cast<bf16*>(A.take(bytes_bf16(BT * I)));
+            }
+            if (t->act8) { k.norm1 = held8(H); k.norm2 = held8(H); k.gate8 = held8(I); k.up8 = held8(I); }
             k.in_rms = static_cast<float*>(A.take(size_t(BT) * 4));
             k.post_rms = static_cast<float*>(A.take(size_t(BT) * 4));
             k.lse = static_cast<float*>(A.take(size_t(BT) * c.q_heads * 4));
@@ -578,6 +628,8 @@ int ta_trainer_tensor(ta_trainer* t, const char* name, void** dev_ptr, long* row
         else if (f == "gate_w") set(w.gate_w, I, H, 1);
         else if (f == "up_w") set(w.up_w, I, H, 1);
         else if (f == "down_w") set(w.down_w, H, I, 1);
+        else if (t->act8 && (f == "cache.x_normed" || f == "cache.r_in" || f == "cache.r_mid"))
+            return fail(t->ctx, TA_ERR_INVALID, std::string("trainer_tensor: not kept with 8-bit activations: ") + name);
         else if (f == "cache.x_normed") set(k.x_normed, BT, H, 1);
         else if (f == "cache.Q") set(k.Q, BT, qd, 1);
         else if (f == "cache.K") set(k.K, BT, kv, 1);

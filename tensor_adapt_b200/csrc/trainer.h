@@ -25,9 +25,15 @@ struct LayerW {
     __nv_bfloat16 *input_norm, *post_norm, *q_w, *k_w, *v_w, *o_w, *q_b, *k_b, *v_b, *gate_w, *up_w, *down_w;
 };
 
+struct Held8 {                    // an activation in 8 bits (act8.cuh)
+    uint8_t *q = nullptr, *scale = nullptr;
+};
+
 struct LayerCache {
+    // with 8-bit activations r_in, r_mid, x_normed, x_normed2, gate, up and act are the same buffers for every layer
     __nv_bfloat16 *r_in, *x_normed, *Q, *K, *V, *attn_out, *r_mid, *x_normed2, *gate, *up, *act;
     float *in_rms, *post_rms, *lse;
+    Held8 norm1, norm2, gate8, up8;   // and these keep the layer's: the two norms before their weights, gate, up
     __nv_bfloat16* h[T_COUNT];   // h_s = bf16(scale * x.A^T) per adapted projection, kept for the backward
 };
 
@@ -58,6 +64,7 @@ struct ta_trainer {
     ta_adapter_config ac{};
     int r_pad = 0;            // rank rounded up to a multiple of 16 (padding rows/columns stay zero)
     float scale = 1.f;        // alpha / rank
+    bool act8 = false;        // activations between forward and backward in 8 bits where an 8-bit form can be read there
     int micro_B = 1, T = 0;   // activation arena is sized for micro_B sequences of T tokens
 
     ta::DeviceArena weights, lora, acts;

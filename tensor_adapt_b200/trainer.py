@@ -122,12 +122,13 @@ class _CudaView:
 class AdaptTrainer:
     def __init__(self, ctx: Context, model: ModelConfig, adapter: AdapterConfig, micro_batch: int, seq_len: int,
                  stream: Optional[int] = None, total_tokens: int = 0, output_dir: Optional[str] = None,
-                 domain: str = "", checkpoint_every: int = 1000):
+                 domain: str = "", checkpoint_every: int = 1000, act_bits: int = 16):
+        """`act_bits` 8 keeps the norms' rows, gate and up in 8 bits between forward and backward (ta_trainer_create_ex)."""
         self.ctx, self.model, self.adapter = ctx, model, adapter
         self.seq_len, self.micro_batch = seq_len, micro_batch
         h = c_void_p()
-        rc = lib.ta_trainer_create(ctx.h, ctypes.byref(model), ctypes.byref(adapter), micro_batch, seq_len,
-                                   c_void_p(stream or 0), ctypes.byref(h))
+        rc = lib.ta_trainer_create_ex(ctx.h, ctypes.byref(model), ctypes.byref(adapter), micro_batch, seq_len, act_bits,
+                                      c_void_p(stream or 0), ctypes.byref(h))
         if rc:
             raise TAError(rc, (lib.ta_last_error(ctx.h) or b"").decode())
         self.h = h

@@ -1,0 +1,111 @@
+"""A training step with 8-bit activations (ta_trainer_create_ex, act_bits 8) against the same step in BF16 and the oracle's.
+
+e4m3 is off by a uniform error of at most half a step, 1/8 / sqrt(12) of a binade in the mean square, 2.46e-2 of a value whose
+fraction is spread over the binade.  A gradient of the last layer has one to three held inputs in its chain (its own, gate, up), one of
+the layer before as many again: sqrt(6) * 2.46e-2 = 0.06; silu' at gate's value moves by up to 1.5 times gate's error: 0.09."""
+import numpy as np
+import pytest
+
+import refcase as rc
+import ta_oracle as o
+
+pytestmark = pytest.mark.gpu
+
+REL = 0.09
+NAMES = ("q", "k", "v", "o", "gate", "up", "down")
+
+
+def run(ctx, cfg, base, adapter, toks, tgts, B, T, bits, targets, micro=None, rank=16, centroid=7, steps=1):
+    from tensor_adapt_b200.trainer import AdaptTrainer, AdapterConfig
+    ac = AdapterConfig.defaults(rank=rank, alpha=32.0, targets=targets, lr=2e-4, centroid_modes=centroid)
+    tr = AdaptTrainer(ctx, rc.model_config(cfg), ac, micro or B, T, act_bits=bits)
+    rc.load_into_trainer(tr, cfg, base, adapter)
+    for s in range(steps):
+        tr.zero_grad()
+        tr.forward_backward(toks[s], tgts[s], B)
+        grads = {(l, n, g): tr.download(f"l{l}.lora.{n}.{g}") for l in range(cfg.layers) for i, n in enumerate(NAMES) if targets >> i & 1 for g in ("gA", "gB")}
+        m = tr.optimizer_step(2e-4)
+    res = {"loss": m.loss, "grads": grads, "flat": tr.download("lora.grad"), "centroid": tr.download("centroid.acc"), "bank": tr.download("centroid_bank.acc")}
+    ctx.check_device()
+    tr.close()
+    return res
+
+
+def rel(a, b):
+    return np.linalg.norm(np.asarray(a, np.float64) - b) / np.linalg.norm(b)
+
+
+@pytest.mark.parametrize("targets", [127, 15, 1 | 64, 2 | 16, 32 | 8])
+def test_step_against_bf16_activations(ctx, targets):
+    cfg = rc.tiny_cfg(hidden=256, hq=4, hkv=2, hd=64, inter=712, layers=2)      # 712: rows that end inside a block
+    B, T, rank = 2, 192, 16
+    names = [n for i, n in enumerate(NAMES) if targets >> i & 1]
+    base, adapter, toks, tgts = rc.make_case(cfg, B, T, rank, targets=names, seed=41, std=0.02, b_std=0.02)
+    a = run(ctx, cfg, base, adapter, toks, tgts, B, T, 8, targets)
+    b = run(ctx, cfg, base, adapter, toks, tgts, B, T, 16, targets)
+    assert abs(a["loss"] - b["loss"]) <= 1e-4 * b["loss"]
+    for k in b["grads"]:
+        assert rel(a["grads"][k], b["grads"][k]) <= REL, k
+    assert rel(a["centroid"], b["centroid"]) <= REL and rel(a["bank"], b["bank"]) <= REL
+    again = run(ctx, cfg, base, adapter, toks, tgts, B, T, 8, targets)
+    assert np.array_equal(a["flat"], again["flat"]) and a["loss"] == again["loss"]
+
+
+def test_gradients_against_the_oracle(ctx):
+    cfg = rc.tiny_cfg(hidden=256, hq=4, hkv=2, hd=64, inter=512, layers=2)
+    B, T, rank = 2, 128, 16
+    base, adapter, toks, tgts = rc.make_case(cfg, B, T, rank, seed=3, std=0.02, b_std=0.02)
+    got = run(ctx, cfg, base, adapter, toks, tgts, B, T, 8, 15, centroid=1)
+    ref = o.train_step(cfg, base, adapter, toks[0], tgts[0], B, T, alpha=32.0, rank=rank, lr=2e-4, step=1, wd=0.0)
+    assert abs(got["loss"] - ref["mean_loss"]) <= 1e-3 * ref["mean_loss"]
+    for l in range(2):
+        for i, n in enumerate("qkvo"):
+            gA, gB = ref["grads"][l * 4 + i]
+            # the BF16 library is within cosine 0.998 (relative 0.063) of the oracle on such a case; the two add in squares
+            for g, r in (("gA", gA), ("gB", gB)):
+                assert rel(got["grads"][l, n, g], r) <= np.hypot(REL, 0.063), (l, n, g)
+
+
+def test_micro_batches_and_a_second_step(ctx):
+    """Five sequences in micro-batches of two (the last one short) accumulate what one batch of five gives; the buffers that all
+    layers share leave nothing of one micro-batch or step for the next."""
+    cfg = rc.tiny_cfg(hidden=128, hq=2, hkv=1, hd=64, inter=328, layers=3)
+    B, T = 5, 64
+    base, adapter, toks, tgts = rc.make_case(cfg, B, T, 16, targets=NAMES, seed=9, std=0.03, b_std=0.03, steps=2)
+    whole = run(ctx, cfg, base, adapter, toks, tgts, B, T, 8, 127, steps=2)
+    parts = run(ctx, cfg, base, adapter, toks, tgts, B, T, 8, 127, micro=2, steps=2)
+    # FP32 sums in another order, and BF16 weights that the first step's Adam moved by a bit the other way
+    assert rel(parts["flat"], whole["flat"]) <= 2e-2 and abs(parts["loss"] - whole["loss"]) <= 1e-4 * whole["loss"]
+
+
+def test_activation_memory(ctx):
+    import torch
+    from tensor_adapt_b200.trainer import AdaptTrainer, AdapterConfig
+    cfg = rc.tiny_cfg(hidden=512, hq=8, hkv=2, hd=64, inter=2048, layers=8)
+    used = {}
+    for bits in (16, 8):
+        torch.cuda.synchronize()
+        before = torch.cuda.mem_get_info()[0]
+        tr = AdaptTrainer(ctx, rc.model_config(cfg), AdapterConfig.defaults(rank=16), 8, 4096, act_bits=bits)
+        used[bits] = before - torch.cuda.mem_get_info()[0]
+        tr.close()
+    BT = 8 * 4096
+    H, I = 512, 2048
+    layer16, layer8 = 2 * (4 * H + 3 * I), (2 * H + 2 * I) * 33 // 32
+    want = BT * (7 * layer16 - 8 * layer8)      # seven of eight layers give up their BF16 buffers, all eight hold 8 bits
+    assert used[16] - used[8] >= want - (64 << 20)
+
+
+def test_refusals(ctx):
+    import tensor_adapt_b200 as ta
+    from tensor_adapt_b200.trainer import AdaptTrainer, AdapterConfig
+    cfg = rc.tiny_cfg()
+    for bits in (0, 4, 32):
+        with pytest.raises(ta.TAError):
+            AdaptTrainer(ctx, rc.model_config(cfg), AdapterConfig.defaults(rank=16), 1, 64, act_bits=bits)
+    tr = AdaptTrainer(ctx, rc.model_config(cfg), AdapterConfig.defaults(rank=16), 1, 64, act_bits=8)
+    for name in ("l0.cache.x_normed", "l1.cache.r_in", "l0.cache.r_mid"):
+        with pytest.raises(ta.TAError):
+            tr.tensor(name)
+    assert tr.tensor("l1.cache.attn_out")[0]
+    tr.close()
