@@ -361,13 +361,13 @@ template <typename F>
 int over_rows(int rows, int D, F launch) {
     Rows r;
     r.nvec = uint32_t(D / 8);
-    r.nblk = uint32_t((D + kQ8Block - 1) / kQ8Block);
+    r.nblk = (uint32_t(D) + kQ8Block - 1) / kQ8Block;
     const uint32_t padded = r.nblk * 4;
     r.padded = FastDiv(padded);
     const int most = std::max(1, int((1u << 30) / padded));
-    for (int at = 0; at < rows; at += most) {
-        r.total = uint32_t(std::min(rows - at, most)) * padded;
-        if (int rc = launch(r, at)) return rc;
+    for (long at = 0; at < rows; at += most) {     // at may pass 2^31
+        r.total = uint32_t(std::min(rows - int(at), most)) * padded;
+        if (int rc = launch(r, int(at))) return rc;
     }
     return TA_OK;
 }
@@ -491,6 +491,7 @@ int ta_add_rms_norm_q8_fwd(ta_ctx* ctx, const void* x, const void* delta, const 
                          aligned16({x, delta, w, res_out, out, q})))
         return rc;
     if (D > 16384) return fail(ctx, TA_ERR_INVALID, "add_rms_norm_q8_fwd: D must be a multiple of 8 and <= 16384");
+    if (reinterpret_cast<uintptr_t>(rms_out) & 3) return fail(ctx, TA_ERR_INVALID, "add_rms_norm_q8_fwd: rms_out must be 4-byte aligned");
     if (rows == 0) return TA_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const auto X = static_cast<const uint4*>(x), De = static_cast<const uint4*>(delta), W = static_cast<const uint4*>(w);
@@ -498,7 +499,7 @@ int ta_add_rms_norm_q8_fwd(ta_ctx* ctx, const void* x, const void* delta, const 
     const auto Q = static_cast<uint2*>(q);
     const auto S = static_cast<uint8_t*>(scale);
 #define TA_LAUNCH(TPR, NV) \
-    add_rms_norm_q8_fwd_kernel<TPR, NV><<<TPR == 32 ? (rows + 3) / 4 : rows, TPR == 32 ? 128 : TPR, 0, s>>>(X, De, W, R, O, Q, S, rms_out, rows, D, 1.0 / D, eps)
+    add_rms_norm_q8_fwd_kernel<TPR, NV><<<TPR == 32 ? (rows - 1) / 4 + 1 : rows, TPR == 32 ? 128 : TPR, 0, s>>>(X, De, W, R, O, Q, S, rms_out, rows, D, 1.0 / D, eps)
     TA_NORM_CASES(TA_LAUNCH, (256, 4), (256, 8));
 #undef TA_LAUNCH
     TA_LAUNCH_CHECK(ctx, "add_rms_norm_q8_fwd_kernel");
@@ -509,6 +510,7 @@ int ta_rms_norm_q8_bwd(ta_ctx* ctx, const void* dy, const void* q, const void* s
                        const void* add_to, int rows, int D, void* stream) {
     if (int rc = q8_args(ctx, "rms_norm_q8_bwd", dy && q && scale && w && rms_saved && dx, rows, D, aligned16({dy, q, w, dx, add_to}))) return rc;
     if (D > 16384) return fail(ctx, TA_ERR_INVALID, "rms_norm_q8_bwd: D must be a multiple of 8 and <= 16384");
+    if (reinterpret_cast<uintptr_t>(rms_saved) & 3) return fail(ctx, TA_ERR_INVALID, "rms_norm_q8_bwd: rms_saved must be 4-byte aligned");
     if (rows == 0) return TA_OK;
     cudaStream_t s = static_cast<cudaStream_t>(stream);
     const auto DY = static_cast<const uint4*>(dy), W = static_cast<const uint4*>(w), AT = static_cast<const uint4*>(add_to);
@@ -516,7 +518,7 @@ int ta_rms_norm_q8_bwd(ta_ctx* ctx, const void* dy, const void* q, const void* s
     const auto S = static_cast<const uint8_t*>(scale);
     const auto DX = static_cast<uint4*>(dx);
 #define TA_LAUNCH(TPR, NV) \
-    rms_norm_q8_bwd_kernel<TPR, NV><<<TPR == 32 ? (rows + 3) / 4 : rows, TPR == 32 ? 128 : TPR, 0, s>>>(DY, Q, S, W, rms_saved, DX, AT, rows, D)
+    rms_norm_q8_bwd_kernel<TPR, NV><<<TPR == 32 ? (rows - 1) / 4 + 1 : rows, TPR == 32 ? 128 : TPR, 0, s>>>(DY, Q, S, W, rms_saved, DX, AT, rows, D)
     TA_NORM_CASES(TA_LAUNCH, (128, 8), (512, 4));
 #undef TA_LAUNCH
     TA_LAUNCH_CHECK(ctx, "rms_norm_q8_bwd_kernel");

@@ -24,6 +24,7 @@
 
 #include <algorithm>
 #include <climits>
+#include <mutex>
 
 #include "act8.cuh"
 #include "ctx.h"
@@ -226,7 +227,7 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
         // small and unaligned for an asynchronous copy: a lane reads the four blocks' bytes of tokens 2t, 2t + 1, 2t + 8 and 2t + 9
         // of a step of 16 (t: lane % 4, the step: lane / 4) one chunk ahead, and stores them as BF16 pairs.  (Two ahead is slower by
         // 1 to 2 us, the lines of L1 that the reads in flight hold are too many.)
-        const int nblk = (N + kQ8Block - 1) / kQ8Block, blk0 = f0 / kQ8Block, me = warp - kConv;
+        const int nblk = int((unsigned(N) + kQ8Block - 1) / kQ8Block), blk0 = f0 / kQ8Block, me = warp - kConv;
         constexpr int kTurn = WIDE ? kLoad : 1;
         const int first = WIDE ? me : 0;
         const bool words = nblk % 4 == 0 && (reinterpret_cast<uintptr_t>(scale) & 3) == 0;    // then so are four blocks of a row
@@ -407,6 +408,7 @@ struct Residency {
     int n[4] = {0, 0, 0, 0};
     bool known = false;
 };
+std::mutex residency_lock;   // contexts of several host threads share the answers
 template <typename F>
 void ask(F kernel, cudaLaunchConfig_t cfg, cudaLaunchAttribute& at, int per_sm, int sm_count, Residency& r) {
     int n[4];
@@ -426,9 +428,7 @@ int launch(const Call& c) {
     using T = Tile<NB, WIDE, RS, BS>;
     ta_ctx* ctx = c.ctx;
     const auto kernel = gemm_tokens_q8_kernel<NB, WIDE, RS, BS>;
-    static Residency resident[64];   // written on first use from the context's one host thread
-    Residency& fit = resident[ctx->device & 63];
-    if (!fit.known) TA_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
+    static Residency resident[64];
     cudaLaunchConfig_t cfg{};
     cfg.blockDim = dim3(T::kThreads);
     cfg.dynamicSmemBytes = T::kSmem;
@@ -438,10 +438,19 @@ int launch(const Call& c) {
     at.val.clusterDim.y = 1; at.val.clusterDim.z = 1;
     cfg.attrs = &at;
     cfg.numAttrs = 1;
-    if (!fit.known) ask(kernel, cfg, at, NB <= 64 ? 2 : 1, ctx->sm_count, fit);
+    Residency fit;
+    {
+        std::lock_guard<std::mutex> hold(residency_lock);
+        Residency& known = resident[ctx->device & 63];
+        if (!known.known) {
+            TA_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
+            ask(kernel, cfg, at, NB <= 64 ? 2 : 1, ctx->sm_count, known);
+        }
+        fit = known;
+    }
     // CTAs on a column tile, 8 (the portable cluster) at most: the fewest rounds of clusters x chunks of a CTA, with what a CTA
     // costs whatever its chunks (8 us; a chunk takes 0.9)
-    const unsigned tiles = unsigned((c.N + kFeat - 1) / kFeat), rows = unsigned((c.M + NB - 1) / NB);
+    const unsigned tiles = (unsigned(c.N) + kFeat - 1) / kFeat, rows = (unsigned(c.M) + NB - 1) / NB;
     const int chunks = (c.K + kTok - 1) / kTok;
     int cs = 0;
     long least = 0;
@@ -479,10 +488,13 @@ extern "C" int ta_gemm_tokens_q8_f32(ta_ctx* ctx, int M, int N, int K, float alp
     if (!ctx || !A || !q || !scale || !C || M <= 0 || N <= 0 || K < 0)
         return fail(ctx, TA_ERR_INVALID, "gemm_tokens_q8_f32: null argument or bad size");
     if (K > INT_MAX - 8 * kTok) return fail(ctx, TA_ERR_UNSUPPORTED, "gemm_tokens_q8_f32: more than 2^31 - 1025 tokens");
+    if (M > 65535 * 128) return fail(ctx, TA_ERR_UNSUPPORTED, "gemm_tokens_q8_f32: more than 65535 * 128 ranks");
     if (M % 8 || N % 8 || lda % 8 || lda < M || ldc < N)
         return fail(ctx, TA_ERR_INVALID, "gemm_tokens_q8_f32: M, N and lda must be multiples of 8, lda >= M, ldc >= N");
     if ((reinterpret_cast<uintptr_t>(A) & 15) || (reinterpret_cast<uintptr_t>(q) & 15))
         return fail(ctx, TA_ERR_INVALID, "gemm_tokens_q8_f32: pointers must be 16-byte aligned");
+    if ((reinterpret_cast<uintptr_t>(C) & 3) || (reinterpret_cast<uintptr_t>(col) & 1))
+        return fail(ctx, TA_ERR_INVALID, "gemm_tokens_q8_f32: C and col must be aligned to their elements");
     if (int rc = on_ctx_device(ctx, "gemm_tokens_q8_f32")) return rc;
     const Call c{ctx, static_cast<cudaStream_t>(stream), static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(scale),
                  static_cast<const __nv_bfloat16*>(A), lda, static_cast<const __nv_bfloat16*>(col), C, ldc, M, N, K, alpha, accumulate};

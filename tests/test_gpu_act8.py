@@ -454,6 +454,91 @@ def test_gradient_shows_a_nan_where_it_is(ctx):
     assert (np.abs(got[:, keep] - A.T @ v) <= grad_bound(A, v, K)).all()
 
 
+@pytest.mark.parametrize("M,N,K", [(16, 128, 300), (64, 384, 1100), (24, 136, 200)])
+def test_gradient_at_odd_addresses(ctx, M, N, K):
+    """scale at an odd address, col and C at their elements' alignment only, C holding NaN before a call that does not accumulate."""
+    ptr, stream_ptr = lib()
+    rng = np.random.default_rng(M * N + K)
+    q, s, A = grad_case(rng, M, N, K)
+    col = r8.bf16(1 + 0.1 * rng.standard_normal(N))
+    v = r8.widen(q, s)
+    for off in (1, 2, 3):
+        sd = torch.full((s.size + off,), 255, dtype=torch.uint8, device="cuda")
+        sd[off:] = raw(s).flatten()
+        cd = torch.full((N + 1,), float("nan"), dtype=torch.bfloat16, device="cuda")
+        cd[1:] = dev(col)
+        C = torch.full((M * N + off,), float("nan"), device="cuda")
+        ctx.call("ta_gemm_tokens_q8_f32", M, N, K, 1.0, ptr(dev(A)), M, ptr(raw(q)), ptr(sd[off:]), ptr(cd[1:]), ptr(C[off:]), N, 0, stream_ptr())
+        got, ref = host(C[off:]).reshape(M, N), (A.T @ v) * col
+        assert (np.abs(got - ref) <= grad_bound(A, v, K) * np.abs(col) + np.abs(ref) * 2 * U).all(), off
+        assert bool(C[:off].isnan().all())
+
+
+def test_contexts_of_two_threads():
+    """Each host thread its own context and stream: the same bits as one thread alone."""
+    import threading
+
+    import tensor_adapt_b200 as ta
+    ptr, _ = lib()
+    rng = np.random.default_rng(12)
+    cases = []
+    for M, N, K in ((16, 904, 2500), (48, 896, 2500), (136, 512, 2500), (64, 3584, 2500)):
+        q, s, A = grad_case(rng, M, N, K)
+        cases.append((M, N, K, raw(q), raw(s), dev(A)))
+    torch.cuda.synchronize()
+    results, faults = [None, None, None], []
+
+    def work(i):
+        try:
+            c, st = ta.Context(), torch.cuda.Stream()
+            with torch.cuda.stream(st):
+                out = [torch.empty(M, N, device="cuda") for M, N, *_ in cases]
+                for _ in range(20):
+                    for (M, N, K, q, s, A), C in zip(cases, out):
+                        c.call("ta_gemm_tokens_q8_f32", M, N, K, 1.0, ptr(A), M, ptr(q), ptr(s), None, ptr(C), N, 0, ta.stream_ptr())
+                st.synchronize()
+            results[i] = out
+        except Exception as e:     # noqa: BLE001 - handed to the test's own thread
+            faults.append(e)
+
+    threads = [threading.Thread(target=work, args=(i,)) for i in range(2)]
+    for t in threads:
+        t.start()
+    for t in threads:
+        t.join()
+    work(2)
+    assert not faults, faults
+    for got in results[:2]:
+        for a, b in zip(got, results[2]):
+            assert torch.equal(a, b)
+
+
+def test_as_many_rows_as_an_int_holds(ctx):
+    """The numbers of rows at which the next piece's first row passes 2^31."""
+    if torch.cuda.get_device_properties(0).total_memory < 100 << 30:
+        pytest.skip("needs 60 GB")
+    ptr, stream_ptr = lib()
+    rows, D = 2 ** 31 - 1, 8
+    x = torch.full((rows * D + 64,), 3.0, dtype=torch.bfloat16, device="cuda")
+    q = torch.full((rows * D + 64,), GUARD, dtype=torch.uint8, device="cuda")
+    s = torch.full((rows + 64,), GUARD, dtype=torch.uint8, device="cuda")
+    x[(rows - 1) * D: rows * D] = 448.0
+    ctx.call("ta_q8_store", ptr(x), ptr(q), ptr(s), rows, D, stream_ptr())
+    three = 3.0 * 2.0 ** 7                                   # the largest power of two that keeps 3 under 448
+    code = int(np.argmin(np.abs(r8.E4M3[:0x7F] - three)))
+    def count(t, value):
+        return sum(int((p == value).sum()) for p in t.split(1 << 30))
+    assert count(q[: (rows - 1) * D], code) == (rows - 1) * D and count(s[: rows - 1], 127 - 7) == rows - 1
+    assert bool((q[(rows - 1) * D: rows * D] == 0x7E).all()) and int(s[rows - 1]) == 127
+    assert bool((q[rows * D:] == GUARD).all()) and bool((s[rows:] == GUARD).all())
+    x[: rows * D].zero_()
+    ctx.call("ta_q8_load", ptr(q), ptr(s), None, ptr(x), rows, D, stream_ptr())
+    assert count(x[: (rows - 1) * D], 3.0) == (rows - 1) * D and bool((x[(rows - 1) * D: rows * D] == 448.0).all())
+    assert bool((x[rows * D:] == 3.0).all())
+    del x, q, s
+    torch.cuda.empty_cache()
+
+
 # ── refusals ────────────────────────────────────────────────────────────────
 
 def test_refusals(ctx):
@@ -488,6 +573,11 @@ def test_refusals(ctx):
         refused("ta_gemm_tokens_q8_f32", M, N, K, 1.0, p, lda, p, p, None, p, ldc, 0, st)
     refused("ta_gemm_tokens_q8_f32", 16, 32, 1, 1.0, odd, 16, p, p, None, p, 32, 0, st)
     refused("ta_gemm_tokens_q8_f32", 16, 32, 1, 1.0, p, 16, odd, p, None, p, 32, 0, st)
+    byte = ptr(b[1:])
+    refused("ta_gemm_tokens_q8_f32", 16, 32, 1, 1.0, p, 16, p, p, None, byte, 32, 0, st)
+    refused("ta_gemm_tokens_q8_f32", 16, 32, 1, 1.0, p, 16, p, p, byte, p, 32, 0, st)
+    refused("ta_add_rms_norm_q8_fwd", p, None, p, None, p, p, p, byte, 1, 32, 1e-6, st)
+    refused("ta_rms_norm_q8_bwd", p, p, p, p, byte, p, None, 1, 32, st)
     torch.cuda.synchronize()
     assert int(b.sum()) == 0
 
