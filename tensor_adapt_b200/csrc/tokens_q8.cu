@@ -358,14 +358,16 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
     for (int o = rank * kThreads + int(threadIdx.x); o < ranks * (kFeat / 4); o += cs * kThreads) {
         const int m = o / (kFeat / 4), c = o % (kFeat / 4) * 4;
         if (f0 + c >= N) continue;                     // N is a multiple of 8: all four or none
-        float4 part[8];
+        float sum[4] = {0.f, 0.f, 0.f, 0.f};
+        for (int from = 0; from < cs; from += 8) {
+            float4 part[8];
 #pragma unroll
-        for (int r = 0; r < 8; r++)
-            if (r < cs) part[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(red, r) + m * kPitch + c);
-        float sum[4] = {part[0].x, part[0].y, part[0].z, part[0].w};
+            for (int r = 0; r < 8; r++)
+                if (from + r < cs) part[r] = *reinterpret_cast<const float4*>(cluster.map_shared_rank(red, from + r) + m * kPitch + c);
 #pragma unroll
-        for (int r = 1; r < 8; r++)
-            if (r < cs) { sum[0] += part[r].x; sum[1] += part[r].y; sum[2] += part[r].z; sum[3] += part[r].w; }
+            for (int r = 0; r < 8; r++)
+                if (from + r < cs) { sum[0] += part[r].x; sum[1] += part[r].y; sum[2] += part[r].z; sum[3] += part[r].w; }
+        }
         float* out = C + size_t(m0 + m) * ldc + f0 + c;
 #pragma unroll
         for (int e = 0; e < 4; e++) {
@@ -401,25 +403,26 @@ struct Call {
     int accumulate;
 };
 
-// Clusters of 1, 2, 4 and 8 CTAs that the device holds at a time, asked once for each kernel and device.  The answer counts one CTA
+// Clusters of 1, 2, 4, 8 and 16 CTAs that the device holds at a time, asked once for each kernel and device.  The answer counts one CTA
 // an SM for these kernels, two of which run on one (NB 64: counters show 24 warps active of 2 x 12); clusters of cs at two CTAs an
 // SM are then as many as clusters of cs / 2 at one.
+constexpr int kSizes = 5;
 struct Residency {
-    int n[4] = {0, 0, 0, 0};
+    int n[kSizes] = {};
     bool known = false;
 };
 std::mutex residency_lock;   // contexts of several host threads share the answers
 template <typename F>
 void ask(F kernel, cudaLaunchConfig_t cfg, cudaLaunchAttribute& at, int per_sm, int sm_count, Residency& r) {
-    int n[4];
-    for (int k = 0; k < 4; k++) {
+    int n[kSizes];
+    for (int k = 0; k < kSizes; k++) {
         at.val.clusterDim.x = 1u << k;
         cfg.gridDim = dim3(1u << k);
         if (cudaOccupancyMaxActiveClusters(&n[k], kernel, &cfg) != cudaSuccess) n[k] = 0;
     }
     (void)cudaGetLastError();
     const bool halved = per_sm == 2 && n[0] <= sm_count;
-    for (int k = 0; k < 4; k++) r.n[k] = !halved ? n[k] : k == 0 ? 2 * n[0] : n[k] > 0 ? n[k - 1] : 0;
+    for (int k = 0; k < kSizes; k++) r.n[k] = !halved ? n[k] : k == 0 ? 2 * n[0] : n[k] > 0 ? n[k - 1] : 0;
     r.known = true;
 }
 
@@ -444,19 +447,21 @@ int launch(const Call& c) {
         Residency& known = resident[ctx->device & 63];
         if (!known.known) {
             TA_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, T::kSmem));
+            TA_CUDA(ctx, cudaFuncSetAttribute(kernel, cudaFuncAttributeNonPortableClusterSizeAllowed, 1));
             ask(kernel, cfg, at, NB <= 64 ? 2 : 1, ctx->sm_count, known);
         }
         fit = known;
     }
-    // CTAs on a column tile, 8 (the portable cluster) at most: the fewest rounds of clusters x chunks of a CTA, with what a CTA
-    // costs whatever its chunks (8 us; a chunk takes 0.9)
+    // CTAs on a column tile: the fewest rounds of clusters x chunks of a CTA, with what a CTA costs whatever its chunks (8 us, 11 in
+    // a cluster of 16; a chunk takes 0.9).  16 against 8, us: 512 columns x 16384 tokens 12.4 / 16.8, 896 x 8192 10.4 / 11.9, 896 x
+    // 2048 7.6 / 7.4, 1536 x 4096 10.7 / 9.0.
     const unsigned tiles = (unsigned(c.N) + kFeat - 1) / kFeat, rows = (unsigned(c.M) + NB - 1) / NB;
     const int chunks = (c.K + kTok - 1) / kTok;
     int cs = 0;
     long least = 0;
-    for (int k = 0; k < 4 && (1 << k) <= chunks; k++) {
+    for (int k = 0; k < kSizes && (1 << k) <= chunks; k++) {
         if (fit.n[k] <= 0) continue;
-        const long rounds = (long(tiles) * rows + fit.n[k] - 1) / fit.n[k], cost = rounds * (((chunks - 1) >> k) + 1 + 8);
+        const long rounds = (long(tiles) * rows + fit.n[k] - 1) / fit.n[k], cost = rounds * (((chunks - 1) >> k) + 1 + (k == 4 ? 11 : 8));
         if (cs == 0 || cost < least) { least = cost; cs = 1 << k; }
     }
     if (cs == 0) return fail(ctx, TA_ERR_CUDA, "gemm_tokens_q8_f32: the kernel cannot be resident on this device");
@@ -487,7 +492,7 @@ extern "C" int ta_gemm_tokens_q8_f32(ta_ctx* ctx, int M, int N, int K, float alp
                                      const void* col, float* C, long ldc, int accumulate, void* stream) {
     if (!ctx || !A || !q || !scale || !C || M <= 0 || N <= 0 || K < 0)
         return fail(ctx, TA_ERR_INVALID, "gemm_tokens_q8_f32: null argument or bad size");
-    if (K > INT_MAX - 8 * kTok) return fail(ctx, TA_ERR_UNSUPPORTED, "gemm_tokens_q8_f32: more than 2^31 - 1025 tokens");
+    if (K > INT_MAX - 64 * kTok) return fail(ctx, TA_ERR_UNSUPPORTED, "gemm_tokens_q8_f32: more than 2^31 - 8193 tokens");
     if (M > 65535 * 128) return fail(ctx, TA_ERR_UNSUPPORTED, "gemm_tokens_q8_f32: more than 65535 * 128 ranks");
     if (M % 8 || N % 8 || lda % 8 || lda < M || ldc < N)
         return fail(ctx, TA_ERR_INVALID, "gemm_tokens_q8_f32: M, N and lda must be multiples of 8, lda >= M, ldc >= N");
