@@ -223,10 +223,11 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
             x_phase ^= 1;
         }
     } else if (warp < kConv + kLoad) {
-        // By TMA the warps take chunks in turn; by cp.async all work on every chunk, and the first has the scales.  Those are too
-        // small and unaligned for an asynchronous copy: a lane reads the four blocks' bytes of tokens 2t, 2t + 1, 2t + 8 and 2t + 9
-        // of a step of 16 (t: lane % 4, the step: lane / 4) one chunk ahead, and stores them as BF16 pairs.  (Two ahead is slower by
-        // 1 to 2 us, the lines of L1 that the reads in flight hold are too many.)
+        // Where q comes by TMA these warps have its scales alone and take chunks in turn; by cp.async all work on every chunk, and the
+        // first has the scales.  Those are too small and unaligned for an asynchronous copy: a lane reads the four blocks' bytes of
+        // tokens 2t, 2t + 1, 2t + 8 and 2t + 9 of a step of 16 (t: lane % 4, the step: lane / 4) one chunk ahead, and stores them as
+        // BF16 pairs.  (Two ahead is slower by 1 to 2 us, the lines of L1 that the reads in flight hold are too many; so is a
+        // prefetch to L2, by 5.)
         const int nblk = int((unsigned(N) + kQ8Block - 1) / kQ8Block), blk0 = f0 / kQ8Block, me = warp - kConv;
         constexpr int kTurn = WIDE ? kLoad : 1;
         const int first = WIDE ? me : 0;
@@ -250,16 +251,11 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
             }
         };
         auto copy = [&](int i, const uint32_t (&h)[4]) {
-            const int rs = i % RS, tok0 = (i * cs + rank) * kTok;
+            const int rs = i % RS;
             if (!warp_wait(&q_empty[rs], (i / RS & 1) ^ 1, DS_TIMEOUT_PRODUCER)) return false;
-            if constexpr (WIDE) {
-                if (lane == 0) {
-                    mbar_arrive_expect_tx(&q_full[rs], T::kQ);
-                    tma_load_2d(smem + rs * T::kQ, &q_map, &q_full[rs], f0, tok0);
-                }
-            } else {
+            if constexpr (!WIDE) {
                 // a lane has eight columns of every 2 kLoad-th token
-                const int f = lane % 16 * 8, tok1 = lane / 16 + 2 * me;
+                const int f = lane % 16 * 8, tok1 = lane / 16 + 2 * me, tok0 = (i * cs + rank) * kTok;
                 const uint8_t* src = q + size_t(tok0 + tok1) * N + f0 + f;
                 const uint32_t dst = base + rs * T::kQ + (f & 8);
 #pragma unroll 4
@@ -290,7 +286,19 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
         }
     } else if (warp == kConv + kLoad) {
         if (lane == 0) {
-            for (int i = 0; i < mine; i++) {
+            // Chunk j of q by TMA, then chunk i of A, as many chunks behind as its ring is shorter: the slot of A is given back
+            // by the products of the chunk whose widening gave back q's.  (q from the warps that have its scales, and so behind
+            // their reads: 1 to 2 % slower.)
+            constexpr int kLag = WIDE ? RS - BS : 0;
+            for (int j = 0; j < mine + kLag; j++) {
+                if (WIDE && j < mine) {
+                    const int rs = j % RS;
+                    if (!mbar_wait(&q_empty[rs], (j / RS & 1) ^ 1, abort_flag, status, DS_TIMEOUT_PRODUCER)) break;
+                    mbar_arrive_expect_tx(&q_full[rs], T::kQ);
+                    tma_load_2d(smem + rs * T::kQ, &q_map, &q_full[rs], f0, (j * cs + rank) * kTok);
+                }
+                const int i = j - kLag;
+                if (i < 0) continue;
                 const int bs = i % BS;
                 if (!mbar_wait(&b_empty[bs], (i / BS & 1) ^ 1, abort_flag, status, DS_TIMEOUT_PRODUCER)) break;
                 mbar_arrive_expect_tx(&b_full[bs], T::kB);
