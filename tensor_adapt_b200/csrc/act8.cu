@@ -322,6 +322,16 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) rms_norm_q8_bwd_kernel(
         b[j] = on ? scale[size_t(row) * nblk + (i >> 2)] : 127;
         a[j] = on && add_to ? add_to[at + i] : make_uint4(0, 0, 0, 0);
     }
+    constexpr bool kEarly = NV <= 2;   // the weights before the sum too, while registers allow it: 1 to 2 us
+    uint4 wv[kEarly ? NV : 1];
+    if constexpr (kEarly) {
+#pragma unroll
+        for (int j = 0; j < NV; j++) wv[j] = lane + j * TPR < nvec ? __ldg(w + lane + j * TPR) : make_uint4(0, 0, 0, 0);
+    }
+    auto weight = [&](int j, float (&f)[8]) {
+        if constexpr (kEarly) unpack8(wv[j], f);
+        else unpack8(__ldg(w + lane + j * TPR), f);
+    };
     float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
@@ -330,7 +340,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) rms_norm_q8_bwd_kernel(
         float fd[8], fn[8], fw[8];
         unpack8(d[j], fd);
         widen8(n[j], b[j], fn);
-        unpack8(__ldg(w + i), fw);
+        weight(j, fw);
 #pragma unroll
         for (int e = 0; e < 8; e++) dot += fd[e] * fw[e] * fn[e];
     }
@@ -343,7 +353,7 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) rms_norm_q8_bwd_kernel(
         float fd[8], fn[8], fw[8], o[8];
         unpack8(d[j], fd);
         widen8(n[j], b[j], fn);
-        unpack8(__ldg(w + i), fw);
+        weight(j, fw);
 #pragma unroll
         for (int e = 0; e < 8; e++) o[e] = rms * (fw[e] * fd[e] - fn[e] * corr);
         if (add_to) {

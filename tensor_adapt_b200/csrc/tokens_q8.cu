@@ -14,12 +14,14 @@
 // tcgen05.mma cuts its sums off instead of rounding them: 8e-6 of the result after 512 products in a row, 1.4e-6 after 128.  So
 // after every four chunks, 32 products, D is added to a running sum beside it, rounded, and starts again (3e-7 in all).
 //
-// What bounds it is the instructions of the widening (issue 70 % busy with two CTAs an SM), 0.9 us a chunk on each of the two, and
-// 8 us whatever the size: launch, first loads, join.  Measured (us; the bytes at the copy rate in parentheses): 16384 tokens x 18944
-// columns, rank 16, 79 (49); 8192 x 8960, rank 64, 27 (12); 8192 x 896, rank 48, 14 (1.3); 8192 x 3584, rank 192, 25 (5).  Other
-// arrangements at the first: mma.sync from registers 66 and at the second 50, where its products alone take 17; the widened
-// operand in shared memory instead, 97 (6 bytes of its traffic an element); q straight to the widening warps' registers, 94 (the
-// proxy fence after a chunk waits for the loads in flight).
+// What bounds it: no single unit (16384 tokens x 18944 columns, rank 16: issue slots 60 % busy, the ALU 42 %, memory 50 %, tensor
+// cores 7 %), but the way of a chunk through them, 1.03 us on each of the two CTAs an SM.  Of 72 us on the device, reading q from
+// memory rather than L2 is 10, the scale bytes 3, the widening 7, the products 9, the rest the barriers between them and 6 to 8 us
+// that any call has: launch, first loads, join.  Measured (us a call; the bytes at the copy rate in parentheses): 16384 x 18944, rank
+// 16, 81 (49); 8192 x 8960, rank 64, 27 (12); 8192 x 896, rank 48, 12 (1.3); 8192 x 3584, rank 192, 25 (5).  Other arrangements at
+// the first: mma.sync from registers 66 and at the second 50, where its products alone take 17; the widened operand in shared memory
+// instead, 97 (6 bytes of its traffic an element); q straight to the widening warps' registers, 94 (the proxy fence after a chunk
+// waits for the loads in flight).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -484,8 +486,8 @@ int launch(const Call& c) {
     TA_LAUNCH_CHECK(ctx, "gemm_tokens_q8_kernel");
     return TA_OK;
 }
-// Rings: with NB 64, 67 KB a CTA leave L1 to the scale reads (four slots of q instead of two: 81 -> 79 us at rank 16, 27 -> 28.5 at
-// rank 64); the larger ones have an SM to themselves.  Above 192 ranks, passes of 128.
+// Rings: with NB 64, 67 KB a CTA leave L1 to the scale reads (four slots of q instead of two, on the device: 72.0 -> 71.3 us at rank
+// 16, 24.5 -> 25.0 at rank 64); the larger ones have an SM to themselves.  Above 192 ranks, passes of 128.
 template <bool WIDE>
 int launch_for_rank(const Call& c) {
     return c.M <= 64 ? launch<64, WIDE, 2, 2>(c) : c.M <= 128 ? launch<128, WIDE, 4, 2>(c) : c.M <= 192 ? launch<192, WIDE, 4, 2>(c) : launch<128, WIDE, 4, 2>(c);

@@ -6,6 +6,7 @@ with ncu; the summaries under profiles/ name the exact command lines).
     python -m tensor_adapt_b200.microbench rowops --rows 16384 --D 3584 --I 18944
     python -m tensor_adapt_b200.microbench lora --BT 4096 --in 896 --out 896 --rank 16
     python -m tensor_adapt_b200.microbench skinny --BT 16384 --in 3584 --out 18944 --rank 16
+    python -m tensor_adapt_b200.microbench act8 --rows 16384 --D 3584 --I 18944 --rank 16
     python -m tensor_adapt_b200.microbench kmeans --N 2048 --D 512 --k 8
 
 Each line reports the median of `--iters` launches after `--warmup`; inputs are larger than L2 or the
@@ -199,10 +200,35 @@ def rowops(ctx, a):
     report("rope", t, bytes_=4.0 * rows * D)
 
 
+def act8(ctx, a):
+    """The entry points that leave or read activations in 8 bits; bytes = every operand once."""
+    rows, D, I, r, e = a.rows, a.D, a.I, a.rank, 1 + 1 / 32      # e: bytes an element in 8 bits
+    def held(cols):
+        return (torch.empty(rows, cols, dtype=torch.uint8, device="cuda"), torch.empty(rows, -(-cols // 32), dtype=torch.uint8, device="cuda"))
+    x, delta, w, dy = rnd(rows, D), rnd(rows, D), rnd(D), rnd(rows, D)
+    res, out = torch.empty_like(x), torch.empty_like(x)
+    rms = torch.empty(rows, device="cuda")
+    (nq, ns), (gq, gs), (uq, us) = held(D), held(I), held(I)
+    g, u, d, dh = rnd(rows, I), rnd(rows, I), rnd(rows, I), rnd(rows, r)
+    o1, o2 = torch.empty_like(g), torch.empty_like(g)
+    gA = torch.zeros(r, I, device="cuda")
+    n = rows * D
+    def run(name, bytes_, *args):
+        t = timeit(lambda: ctx.call("ta_" + name, *args, stream_ptr()), a.iters, a.warmup, a.flush)
+        report(name, t, bytes_=bytes_)
+    run("q8_store", n * (2 + e), ptr(x), ptr(nq), ptr(ns), rows, D)
+    run("q8_load", n * (2 + e), ptr(nq), ptr(ns), ptr(w), ptr(out), rows, D)
+    run("add_rms_norm_q8_fwd", n * (8 + e), ptr(x), ptr(delta), ptr(w), ptr(res), ptr(out), ptr(nq), ptr(ns), ptr(rms), rows, D, 1e-6)
+    run("rms_norm_q8_bwd", n * (6 + e), ptr(dy), ptr(nq), ptr(ns), ptr(w), ptr(rms), ptr(out), ptr(res), rows, D)
+    run("silu_mul_q8_fwd", rows * I * (6 + 2 * e), ptr(g), ptr(u), ptr(o1), ptr(gq), ptr(gs), ptr(uq), ptr(us), rows, I)
+    run("silu_mul_q8_bwd", rows * I * (8 + 2 * e), ptr(d), ptr(gq), ptr(gs), ptr(uq), ptr(us), ptr(o1), ptr(o2), ptr(g), rows, I)
+    run("gemm_tokens_q8_f32", rows * (I * e + 2 * r) + 4 * r * I, r, I, rows, 1.0, ptr(dh), r, ptr(uq), ptr(us), None, ptr(gA), I, 0)
+
+
 def main():
     ap = argparse.ArgumentParser()
     sub = ap.add_subparsers(dest="what", required=True)
-    for name in ("attention", "gemm", "lora", "rowops", "skinny", "kmeans", "swiglu"):
+    for name in ("attention", "gemm", "lora", "rowops", "skinny", "kmeans", "swiglu", "act8"):
         s = sub.add_parser(name)
         s.add_argument("--iters", type=int, default=10); s.add_argument("--warmup", type=int, default=3)
         s.add_argument("--flush", action="store_true")
@@ -225,11 +251,13 @@ def main():
         else:
             for k, v in (("rows", 16384), ("D", 3584), ("I", 18944)):
                 s.add_argument("--" + k, type=int, default=v)
+            if name == "act8":
+                s.add_argument("--rank", type=int, default=16)
             if name == "swiglu":
                 s.add_argument("--pair", type=int, default=0)
     a = ap.parse_args()
     ctx = ta.Context(0)
-    {"attention": attention, "gemm": gemm, "lora": lora, "rowops": rowops, "skinny": skinny, "kmeans": kmeans, "swiglu": swiglu}[a.what](ctx, a)
+    {"attention": attention, "gemm": gemm, "lora": lora, "rowops": rowops, "skinny": skinny, "kmeans": kmeans, "swiglu": swiglu, "act8": act8}[a.what](ctx, a)
     torch.cuda.synchronize()
     ctx.check_device()
 
