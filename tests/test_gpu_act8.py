@@ -686,6 +686,59 @@ def test_capture_and_replay_on_a_second_stream(ctx):
             assert torch.equal(a[k], eager[k]), k
 
 
+FIRST_CALLS = """
+import torch
+import tensor_adapt_b200 as ta
+from tensor_adapt_b200 import ptr, stream_ptr
+ctx = ta.Context(0)
+torch.manual_seed(0)
+BT, H, r = 700, 904, 24
+bf = lambda *s: torch.randn(*s, device="cuda").to(torch.bfloat16)
+by = lambda n: torch.zeros(BT, n, dtype=torch.uint8, device="cuda")
+x, d, w, g, u, dy, dh = bf(BT, H), bf(BT, H), bf(H), bf(BT, H), bf(BT, H), bf(BT, H), bf(BT, r)
+def outputs():
+    o = {k: torch.zeros(BT, H, dtype=torch.bfloat16, device="cuda") for k in ("res", "n", "act", "dg", "du", "act2", "dx", "back")}
+    o.update({k: by(H) for k in ("nq", "gq", "uq", "aq")})
+    o.update({k: by(-(-H // 32)) for k in ("ns", "gs", "us", "as")})
+    o.update(rms=torch.zeros(BT, device="cuda"), gA=torch.zeros(r, H, device="cuda"), gW=torch.zeros(r, 896, device="cuda"))
+    return o
+wide, wide_s = torch.full((BT, 896), 0x38, dtype=torch.uint8, device="cuda"), torch.full((BT, 28), 127, dtype=torch.uint8, device="cuda")
+def calls(o):
+    p, st = {k: ptr(v) for k, v in o.items()}, stream_ptr()
+    ctx.call("ta_add_rms_norm_q8_fwd", ptr(x), ptr(d), ptr(w), p["res"], p["n"], p["nq"], p["ns"], p["rms"], BT, H, 1e-6, st)
+    ctx.call("ta_silu_mul_q8_fwd", ptr(g), ptr(u), p["act"], p["gq"], p["gs"], p["uq"], p["us"], BT, H, st)
+    ctx.call("ta_silu_mul_q8_bwd", ptr(dy), p["gq"], p["gs"], p["uq"], p["us"], p["dg"], p["du"], p["act2"], BT, H, st)
+    ctx.call("ta_q8_store", p["act2"], p["aq"], p["as"], BT, H, st)
+    ctx.call("ta_q8_load", p["aq"], p["as"], None, p["back"], BT, H, st)
+    ctx.call("ta_gemm_tokens_q8_f32", r, H, BT, 1.0, ptr(dh), r, p["nq"], p["ns"], ptr(w), p["gA"], H, 0, st)
+    ctx.call("ta_gemm_tokens_q8_f32", r, 896, BT, 1.0, ptr(dh), r, ptr(wide), ptr(wide_s), None, p["gW"], 896, 0, st)
+    ctx.call("ta_rms_norm_q8_bwd", ptr(dy), p["nq"], p["ns"], ptr(w), p["rms"], p["dx"], ptr(x), BT, H, st)
+a, b = outputs(), outputs()
+torch.cuda.synchronize()
+graph = torch.cuda.CUDAGraph()
+with torch.cuda.graph(graph):
+    calls(a)
+assert all(not bool(v.any()) for v in a.values())
+graph.replay()
+calls(b)
+torch.cuda.synchronize()
+assert all(torch.equal(a[k], b[k]) for k in a), [k for k in a if not torch.equal(a[k], b[k])]
+assert all(bool(v.any()) for v in b.values())
+ctx.check_device()
+print("captured")
+"""
+
+
+def test_first_calls_of_a_process_are_captured():
+    """Nothing has to be warmed up: the very first call of every entry point may be inside a capture."""
+    import os
+    import subprocess
+    import sys
+    root = os.path.dirname(os.path.dirname(os.path.abspath(__file__)))
+    done = subprocess.run([sys.executable, "-c", FIRST_CALLS], cwd=root, capture_output=True, text=True, timeout=300)
+    assert done.returncode == 0 and "captured" in done.stdout, done.stderr[-2000:]
+
+
 def test_two_streams_at_once(ctx):
     ptr, stream_ptr = lib()
     rng = np.random.default_rng(6)
