@@ -40,7 +40,7 @@ static EncodeTiledFn encode_fn() {
 }
 
 int encode_tmap_2d(ta_ctx* ctx, CUtensorMapDataType type, const void* ptr, uint64_t dim0, uint64_t dim1, uint64_t pitch_bytes,
-                   uint32_t box0, uint32_t box1, int span, CUtensorMap* out) {
+                   uint32_t box0, uint32_t box1, int span, CUtensorMap* out, bool wide_l2) {
     EncodeTiledFn fn = encode_fn();
     if (!fn) return fail(ctx, TA_ERR_CUDA, "cuTensorMapEncodeTiled is not available from this driver");
     if ((reinterpret_cast<uintptr_t>(ptr) & 15) || (pitch_bytes & 15))
@@ -52,7 +52,7 @@ int encode_tmap_2d(ta_ctx* ctx, CUtensorMapDataType type, const void* ptr, uint6
     const CUtensorMapSwizzle swz = span == 128 ? CU_TENSOR_MAP_SWIZZLE_128B : span == 64 ? CU_TENSOR_MAP_SWIZZLE_64B
                                  : span == 32 ? CU_TENSOR_MAP_SWIZZLE_32B : CU_TENSOR_MAP_SWIZZLE_NONE;
     CUresult r = fn(out, type, 2, const_cast<void*>(ptr), gdim, gstride, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE, swz,
-                    CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+                    wide_l2 ? CU_TENSOR_MAP_L2_PROMOTION_L2_256B : CU_TENSOR_MAP_L2_PROMOTION_L2_128B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) {
         char buf[200];
         std::snprintf(buf, sizeof(buf), "cuTensorMapEncodeTiled failed (%d) dims=%llu x %llu pitch=%llu box=%u x %u",

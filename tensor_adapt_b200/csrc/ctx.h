@@ -92,9 +92,9 @@ int encode_tmap_bf16(ta_ctx* ctx, const void* ptr, uint64_t dim0, uint64_t dim1,
                      uint32_t box1, CUtensorMap* out);
 
 // 2-D map of any element type, not cached: dim0 elements a row, dim1 rows, box box0 x box1, `span` the swizzle's 32, 64 or 128
-// bytes (the box's inner extent) or 0 for none; elements outside read as zero.
+// bytes (the box's inner extent) or 0 for none; elements outside read as zero.  wide_l2: misses fetch 256 bytes to L2, not 128.
 int encode_tmap_2d(ta_ctx* ctx, CUtensorMapDataType type, const void* ptr, uint64_t dim0, uint64_t dim1, uint64_t pitch_bytes,
-                   uint32_t box0, uint32_t box1, int span, CUtensorMap* out);
+                   uint32_t box0, uint32_t box1, int span, CUtensorMap* out, bool wide_l2 = true);
 
 // Scratch of at least `bytes`, grown on demand when the context owns its workspace.
 int get_workspace(ta_ctx* ctx, size_t bytes, void** out);

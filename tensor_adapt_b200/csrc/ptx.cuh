@@ -354,14 +354,18 @@ __device__ __forceinline__ void umma_commit_pair(uint32_t bar_cluster_addr) {
 // MN-major operand (each K index is one 128-B row holding 64 consecutive M/N elements, the layout a
 //   TMA box {64 mn, 64 k} produces): 8-k groups are 1024 B apart (SBO = 1024), consecutive 64-wide
 //   M/N chunks are `lbo` bytes apart (one box = 8192 B).  Advancing K by one MMA adds 2048 B.
-__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+// Narrower MN-major rows of 64 or 32 bytes (32 or 16 elements) the same way, swizzled over their span.
+__device__ __forceinline__ uint64_t smem_desc(int span, uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
     uint64_t d = 0;
     d |= static_cast<uint64_t>((saddr & 0x3FFFFu) >> 4);
     d |= static_cast<uint64_t>((lbo_bytes >> 4) & 0x3FFFu) << 16;
     d |= static_cast<uint64_t>((sbo_bytes >> 4) & 0x3FFFu) << 32;
     d |= 1ull << 46;
-    d |= 2ull << 61;
+    d |= (span == 128 ? 2ull : span == 64 ? 4ull : 6ull) << 61;
     return d;
+}
+__device__ __forceinline__ uint64_t smem_desc_sw128(uint32_t saddr, uint32_t lbo_bytes, uint32_t sbo_bytes) {
+    return smem_desc(128, saddr, lbo_bytes, sbo_bytes);
 }
 
 // Instruction descriptor for kind::f16 with BF16 A/B and FP32 D:

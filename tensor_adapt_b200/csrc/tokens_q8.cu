@@ -14,14 +14,14 @@
 // tcgen05.mma cuts its sums off instead of rounding them: 8e-6 of the result after 512 products in a row, 1.4e-6 after 128.  So
 // after every four chunks, 32 products, D is added to a running sum beside it, rounded, and starts again (3e-7 in all).
 //
-// What bounds it: no single unit (16384 tokens x 18944 columns, rank 16: issue slots 60 % busy, the ALU 42 %, memory 50 %, tensor
-// cores 7 %), but the way of a chunk through them, 1.03 us on each of the two CTAs an SM.  Of 72 us on the device, reading q from
-// memory rather than L2 is 10, the scale bytes 3, the widening 7, the products 9, the rest the barriers between them and 6 to 8 us
-// that any call has: launch, first loads, join.  Measured (us a call; the bytes at the copy rate in parentheses): 16384 x 18944, rank
-// 16, 81 (49); 8192 x 8960, rank 64, 27 (12); 8192 x 896, rank 48, 12 (1.3); 8192 x 3584, rank 192, 25 (5).  Other arrangements at
-// the first: mma.sync from registers 66 and at the second 50, where its products alone take 17; the widened operand in shared memory
-// instead, 97 (6 bytes of its traffic an element); q straight to the widening warps' registers, 94 (the proxy fence after a chunk
-// waits for the loads in flight).
+// What bounds it, at 16384 tokens x 18944 columns and rank 16: the way of q through memory (5.5 TB/s while it runs), with the scale
+// bytes beside it, of whose 32-byte sectors a tile uses four.  In-kernel clocks show the widening warps waiting for data most of the
+// time; issue slots are 60 % busy, the ALU 42 %, the tensor cores 7 %.  6 to 8 us any call has: launch, first loads, join.  Measured
+// (us a call; the bytes at the copy rate in parentheses): 16384 x 18944, rank 16, 75 (49); 8192 x 8960, rank 64, 28 (12); 8192 x 896,
+// rank 48, 12 (1.3); 8192 x 3584, rank 192, 25 (5).  Other arrangements at the first, on the device, where this one takes 63: mma.sync
+// from registers 66 and at the second 50, where its products alone take 17; the widened operand in shared memory instead, 97 (6 bytes
+// of its traffic an element); q straight to the widening warps' registers, 94 (the proxy fence after a chunk waits for the loads in
+// flight).
 #include <cooperative_groups.h>
 
 #include <algorithm>
@@ -42,7 +42,7 @@ constexpr int kPitch = kFeat + 4;           // of the sums in shared memory
 
 constexpr int kRun = 4;                     // chunks that D takes in a row
 
-// NB: room for ranks, 64, 128 or 192.  Rings: RS chunks of q and scales, BS of A's rows, two of the widened operand.  The sets of
+// NB: room for ranks, 16, 32, 64, 128 or 192.  Rings: RS chunks of q and scales, BS of A's rows, two of the widened operand.  The sets of
 // widening warps and the loaders of the TMA form take chunks in turn.  A wait on a barrier's parity cannot tell phases two apart, so
 // nobody may come to a slot whose phase before last is not complete: with an even ring and two of each, a slot is always the same
 // set's and the same loader's, which has waited for that phase itself.
@@ -51,8 +51,9 @@ template <int NB, bool WIDE, int RS, int BS>
 struct Tile {
     static constexpr int kLoad = WIDE ? 2 : 6, kThreads = 32 * (kConv + kLoad + 2);
     static_assert(RS % 2 == 0, "");
-    static constexpr int kBoxes = NB / 64;                          // of A, 64 ranks (128 bytes) wide
-    static constexpr int kQ = kFeat * kTok, kBox = kTok * 128, kB = kBoxes * kBox;
+    static constexpr int kWide = NB < 64 ? NB : 64, kRow = 2 * kWide; // of a box of A: ranks, bytes
+    static constexpr int kBoxes = NB / kWide;
+    static constexpr int kQ = kFeat * kTok, kBox = kTok * kRow, kB = kBoxes * kBox;
     static constexpr int kScale = kTok * (kFeat / kQ8Block) * 2;     // as BF16
     static constexpr int kAtB = RS * kQ, kAtS = kAtB + BS * kB;
     static constexpr int kRings = kAtS + RS * kScale, kRed = NB * kPitch * 4;
@@ -115,9 +116,17 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
     const int f0 = int(blockIdx.x) / cs * kFeat, m0 = int(blockIdx.y) * NB;
     const int chunks = (K + kTok - 1) / kTok;
     const int mine = chunks > rank ? (chunks - rank + cs - 1) / cs : 0;   // chunks rank, rank + cs, ...
-    if (threadIdx.x == 0) {
-        if (WIDE) prefetch_tensormap(&q_map);
-        prefetch_tensormap(&a_map);
+    auto copy_q = [&](int j) {
+        mbar_arrive_expect_tx(&q_full[j % RS], T::kQ);
+        tma_load_2d(smem + j % RS * T::kQ, &q_map, &q_full[j % RS], f0, (j * cs + rank) * kTok);
+    };
+    auto copy_a = [&](int i) {
+        mbar_arrive_expect_tx(&b_full[i % BS], T::kB);
+#pragma unroll
+        for (int c = 0; c < T::kBoxes; c++)
+            tma_load_2d(smem + T::kAtB + i % BS * T::kB + c * T::kBox, &a_map, &b_full[i % BS], m0 + T::kWide * c, (i * cs + rank) * kTok);
+    };
+    if (threadIdx.x == 32 * (kConv + kLoad)) {
         for (int i = 0; i < RS; i++) {
             mbar_init(&q_full[i], WIDE ? 2 : 1 + 32 * kLoad);
             mbar_init(&q_empty[i], kConv / 2);
@@ -135,7 +144,41 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
         mbar_init(&done, 1);
         abort_word = 0;
         fence_barrier_init();
+        fence_proxy_async_smem();
+        // the first round of the rings: this thread's copies need nobody else
+        for (int i = 0; i < RS && i < mine; i++) {
+            if (WIDE) copy_q(i);
+            if (i < BS) copy_a(i);
+        }
     }
+    // Where q comes by TMA the loaders have its scales alone and take chunks in turn; by cp.async all work on every chunk, and the
+    // first has the scales.  Those are too small and unaligned for an asynchronous copy: a lane reads the four blocks' bytes of
+    // tokens 2t, 2t + 1, 2t + 8 and 2t + 9 of a step of 16 (t: lane % 4, the step: lane / 4) one chunk ahead, and stores them as
+    // BF16 pairs.  (Two ahead is slower by 1 to 2 us, the lines of L1 that the reads in flight hold are too many; so is a prefetch
+    // to L2, by 5.)
+    const int nblk = int((unsigned(N) + kQ8Block - 1) / kQ8Block), blk0 = f0 / kQ8Block, me = warp - kConv;
+    constexpr int kTurn = WIDE ? kLoad : 1;
+    const int first = WIDE ? me : 0;
+    const bool words = nblk % 4 == 0 && (reinterpret_cast<uintptr_t>(scale) & 3) == 0;    // then so are four blocks of a row
+    uint32_t held[4];
+    auto read = [&](int i, uint32_t (&h)[4]) {
+        const int tok0 = (i * cs + rank) * kTok + (lane >> 2) * 16 + (lane & 3) * 2;
+#pragma unroll
+        for (int j = 0; j < 4; j++) {
+            const int tok = tok0 + (j & 1) + (j >> 1) * 8;
+            h[j] = 0x7F7F7F7Fu;
+            if (i >= mine || tok >= K || (!WIDE && me != 0)) continue;
+            const uint8_t* p = scale + size_t(tok) * nblk + blk0;
+            if (words) {
+                h[j] = __ldg(reinterpret_cast<const uint32_t*>(p));
+            } else {
+#pragma unroll
+                for (int b = 0; b < 4; b++)
+                    if (blk0 + b < nblk) h[j] = (h[j] & ~(0xFFu << 8 * b)) | uint32_t(p[b]) << 8 * b;
+            }
+        }
+    };
+    if (warp >= kConv && warp < kConv + kLoad) read(first, held);
     if (warp == kConv + kLoad + 1) {
         tmem_alloc(&tmem_slot, T::kTmem);
         tmem_relinquish();
@@ -225,33 +268,6 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
             x_phase ^= 1;
         }
     } else if (warp < kConv + kLoad) {
-        // Where q comes by TMA these warps have its scales alone and take chunks in turn; by cp.async all work on every chunk, and the
-        // first has the scales.  Those are too small and unaligned for an asynchronous copy: a lane reads the four blocks' bytes of
-        // tokens 2t, 2t + 1, 2t + 8 and 2t + 9 of a step of 16 (t: lane % 4, the step: lane / 4) one chunk ahead, and stores them as
-        // BF16 pairs.  (Two ahead is slower by 1 to 2 us, the lines of L1 that the reads in flight hold are too many; so is a
-        // prefetch to L2, by 5.)
-        const int nblk = int((unsigned(N) + kQ8Block - 1) / kQ8Block), blk0 = f0 / kQ8Block, me = warp - kConv;
-        constexpr int kTurn = WIDE ? kLoad : 1;
-        const int first = WIDE ? me : 0;
-        const bool words = nblk % 4 == 0 && (reinterpret_cast<uintptr_t>(scale) & 3) == 0;    // then so are four blocks of a row
-        uint32_t held[4];
-        auto read = [&](int i, uint32_t (&h)[4]) {
-            const int tok0 = (i * cs + rank) * kTok + (lane >> 2) * 16 + (lane & 3) * 2;
-#pragma unroll
-            for (int j = 0; j < 4; j++) {
-                const int tok = tok0 + (j & 1) + (j >> 1) * 8;
-                h[j] = 0x7F7F7F7Fu;
-                if (i >= mine || tok >= K || (!WIDE && me != 0)) continue;
-                const uint8_t* p = scale + size_t(tok) * nblk + blk0;
-                if (words) {
-                    h[j] = __ldg(reinterpret_cast<const uint32_t*>(p));
-                } else {
-#pragma unroll
-                    for (int b = 0; b < 4; b++)
-                        if (blk0 + b < nblk) h[j] = (h[j] & ~(0xFFu << 8 * b)) | uint32_t(p[b]) << 8 * b;
-                }
-            }
-        };
         auto copy = [&](int i, const uint32_t (&h)[4]) {
             const int rs = i % RS;
             if (!warp_wait(&q_empty[rs], (i / RS & 1) ^ 1, DS_TIMEOUT_PRODUCER)) return false;
@@ -281,7 +297,6 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
             if (lane == 0) mbar_arrive(&q_full[rs]);
             return true;
         };
-        read(first, held);
         for (int i = first; i < mine; i += kTurn) {
             if (!copy(i, held)) break;
             read(i + kTurn, held);
@@ -292,21 +307,14 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
             // by the products of the chunk whose widening gave back q's.  (q from the warps that have its scales, and so behind
             // their reads: 1 to 2 % slower.)
             constexpr int kLag = WIDE ? RS - BS : 0;
-            for (int j = 0; j < mine + kLag; j++) {
+            for (int j = BS + kLag; j < mine + kLag; j++) {      // BS + kLag is RS where q comes by TMA
                 if (WIDE && j < mine) {
-                    const int rs = j % RS;
-                    if (!mbar_wait(&q_empty[rs], (j / RS & 1) ^ 1, abort_flag, status, DS_TIMEOUT_PRODUCER)) break;
-                    mbar_arrive_expect_tx(&q_full[rs], T::kQ);
-                    tma_load_2d(smem + rs * T::kQ, &q_map, &q_full[rs], f0, (j * cs + rank) * kTok);
+                    if (!mbar_wait(&q_empty[j % RS], (j / RS & 1) ^ 1, abort_flag, status, DS_TIMEOUT_PRODUCER)) break;
+                    copy_q(j);
                 }
                 const int i = j - kLag;
-                if (i < 0) continue;
-                const int bs = i % BS;
-                if (!mbar_wait(&b_empty[bs], (i / BS & 1) ^ 1, abort_flag, status, DS_TIMEOUT_PRODUCER)) break;
-                mbar_arrive_expect_tx(&b_full[bs], T::kB);
-#pragma unroll
-                for (int c = 0; c < T::kBoxes; c++)
-                    tma_load_2d(smem + T::kAtB + bs * T::kB + c * T::kBox, &a_map, &b_full[bs], m0 + 64 * c, (i * cs + rank) * kTok);
+                if (!mbar_wait(&b_empty[i % BS], (i / BS & 1) ^ 1, abort_flag, status, DS_TIMEOUT_PRODUCER)) break;
+                copy_a(i);
             }
         }
     } else if (lane == 0) {
@@ -318,9 +326,9 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
             if (ok && i > 0 && i % kRun == 0) ok = mbar_wait(&d_empty, (i / kRun - 1) & 1, abort_flag, status, DS_TIMEOUT_MMA);
             if (!ok) break;
             tcgen05_fence_after_sync();
-            const uint64_t bd = smem_desc_sw128(base + T::kAtB + bs * T::kB, T::kBox, 1024);
+            const uint64_t bd = smem_desc(T::kRow, base + T::kAtB + bs * T::kB, T::kBox, 8 * T::kRow);
 #pragma unroll
-            for (int k = 0; k < kTok / 16; k++) umma_bf16_ts(d_tmem, x_tmem + xs * T::kX + k * 8, bd + k * (2048 >> 4), idesc, uint32_t(i % kRun + k > 0));
+            for (int k = 0; k < kTok / 16; k++) umma_bf16_ts(d_tmem, x_tmem + xs * T::kX + k * 8, bd + k * T::kRow, idesc, uint32_t(i % kRun + k > 0));
             umma_commit(&x_empty[xs]);
             umma_commit(&b_empty[bs]);
             if (i % kRun == kRun - 1 && i + 1 < mine) umma_commit(&d_full);
@@ -414,7 +422,7 @@ struct Call {
 };
 
 // Clusters of 1, 2, 4, 8 and 16 CTAs that the device holds at a time, asked once for each kernel and device.  The answer counts one CTA
-// an SM for these kernels, two of which run on one (NB 64: counters show 24 warps active of 2 x 12); clusters of cs at two CTAs an
+// an SM for these kernels, two of which run on one (NB <= 64: counters show 24 warps active of 2 x 12); clusters of cs at two CTAs an
 // SM are then as many as clusters of cs / 2 at one.
 constexpr int kSizes = 5;
 struct Residency {
@@ -479,18 +487,21 @@ int launch(const Call& c) {
     cfg.gridDim = dim3(tiles * unsigned(cs), rows);
     CUtensorMap q_map{}, a_map;
     if (WIDE)
-        if (int rc = encode_tmap_2d(ctx, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.q, c.N, c.K, c.N, kFeat, kTok, 128, &q_map)) return rc;
-    if (int rc = encode_tmap_2d(ctx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c.A, c.M, c.K, c.lda * 2, 64, kTok, 128, &a_map)) return rc;
+        if (int rc = encode_tmap_2d(ctx, CU_TENSOR_MAP_DATA_TYPE_UINT8, c.q, c.N, c.K, c.N, kFeat, kTok, 128, &q_map, false)) return rc;
+    if (int rc = encode_tmap_2d(ctx, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, c.A, c.M, c.K, c.lda * 2, T::kWide, kTok, T::kRow, &a_map)) return rc;
     ProfScope prof(ctx, c.stream, PROF_GEMM_SKINNY, 2.0 * c.M * c.N * c.K);
     TA_CUDA(ctx, cudaLaunchKernelEx(&cfg, kernel, q_map, a_map, c.q, c.scale, c.col, c.C, c.ldc, c.M, c.N, c.K, c.alpha, c.accumulate, ctx->d_status));
     TA_LAUNCH_CHECK(ctx, "gemm_tokens_q8_kernel");
     return TA_OK;
 }
-// Rings: with NB 64, 67 KB a CTA leave L1 to the scale reads (four slots of q instead of two, on the device: 72.0 -> 71.3 us at rank
-// 16, 24.5 -> 25.0 at rank 64); the larger ones have an SM to themselves.  Above 192 ranks, passes of 128.
+// Room for 16 or 32 ranks beside 64: boxes of A as wide as they, since a box is filled whatever the rank (16384 x 18944, rank 16, us on
+// the device: 62.7 against 70.2; rank 32 65.3).  Rings: four slots of q by TMA (two: 72 at rank 16, and 78 against 74 at rank 64); two
+// by cp.async, where L1 and not the latency is short (8960 x 8192, rank 64: 31.7, with four 36.5).  Above 192 ranks, passes of 128.
 template <bool WIDE>
 int launch_for_rank(const Call& c) {
-    return c.M <= 64 ? launch<64, WIDE, 2, 2>(c) : c.M <= 128 ? launch<128, WIDE, 4, 2>(c) : c.M <= 192 ? launch<192, WIDE, 4, 2>(c) : launch<128, WIDE, 4, 2>(c);
+    constexpr int RS = WIDE ? 4 : 2;
+    return c.M <= 16 ? launch<16, WIDE, RS, 2>(c) : c.M <= 32 ? launch<32, WIDE, RS, 2>(c) : c.M <= 64 ? launch<64, WIDE, RS, 2>(c)
+         : c.M <= 128 ? launch<128, WIDE, 4, 2>(c) : c.M <= 192 ? launch<192, WIDE, 4, 2>(c) : launch<128, WIDE, 4, 2>(c);
 }
 
 }  // namespace
