@@ -404,7 +404,9 @@ __global__ void __launch_bounds__(Tile<NB, WIDE, RS, BS>::kThreads, NB <= 64 ? 2
             for (int e = 0; e < 4; e++) out[e] = accumulate ? out[e] + sum[e] : sum[e];
         }
     }
-    cluster.sync();   // nobody leaves while its sums are read
+    // Nobody leaves while its sums are read.  A relaxed arrival does not wait for the stores above (0.2 to 0.3 us); the reads are done,
+    // since the stores take their values.
+    asm volatile("barrier.cluster.arrive.relaxed;\nbarrier.cluster.wait;" ::: "memory");
 }
 
 struct Call {
