@@ -483,16 +483,20 @@ int ta_silu_mul_q8_bwd(ta_ctx* ctx, const void* dout, const void* gate_q, const 
 // at the longest row of the class; in parentheses the next best): 64 x 2 at 1024 columns 26.9 / 22.7 (a warp 28.3 / 25.0), 128 x 2
 // at 2048 49.4 / 39.6 (64 x 4 49.8 / 42.3), 128 x 4 at 3584 83.6 / 67.3 (256 x 2 82.8 / 70.1), at 8192 forward 256 x 4 183 (128 x 8
 // 185) and backward, which holds three arrays, 128 x 8 154 (256 x 4 168).
-#define TA_NORM_CASES(LAUNCH, AT_8192, AT_16384)               \
-    do {                                                       \
-        const int nvec = D / 8;                                \
-        if (nvec <= 32)        LAUNCH(32, 1);                  \
-        else if (nvec <= 64)   LAUNCH(32, 2);                  \
-        else if (nvec <= 128)  LAUNCH(64, 2);                  \
-        else if (nvec <= 256)  LAUNCH(128, 2);                 \
-        else if (nvec <= 512)  LAUNCH(128, 4);                 \
-        else if (nvec <= 1024) LAUNCH AT_8192;                 \
-        else                   LAUNCH AT_16384;                \
+// Few rows, up to four an SM, leave most of the device idle and are bound by a row's own latency: more threads a row then (us,
+// forward / backward, from L2: 1 x 896 1.7 / 1.5, with the others 2.1 / 1.6; 256 x 3584 2.9 / 2.8, 3.8 / 3.3; 64 x 8192 3.2 / 2.8, 3.8 /
+// 4.5; 592 x 8192 11.3 / 10.0, 9.6 / 14.3; beyond, at 1024 x 3584, 8.8 / 7.0, 7.8 / 8.7).
+#define TA_NORM_CASES(LAUNCH, AT_8192, AT_16384)                                        \
+    do {                                                                                \
+        const int nvec = D / 8;                                                         \
+        const bool few = rows <= 4 * ctx->sm_count;                                     \
+        if (nvec <= 32)        LAUNCH(32, 1);                                           \
+        else if (nvec <= 64)   LAUNCH(32, 2);                                           \
+        else if (nvec <= 128)  { if (few) LAUNCH(128, 1); else LAUNCH(64, 2); }         \
+        else if (nvec <= 256)  { if (few) LAUNCH(256, 1); else LAUNCH(128, 2); }        \
+        else if (nvec <= 512)  { if (few) LAUNCH(512, 1); else LAUNCH(128, 4); }        \
+        else if (nvec <= 1024) { if (few) LAUNCH(512, 2); else LAUNCH AT_8192; }        \
+        else                   { if (few) LAUNCH(512, 4); else LAUNCH AT_16384; }       \
     } while (0)
 
 int ta_add_rms_norm_q8_fwd(ta_ctx* ctx, const void* x, const void* delta, const void* w, void* res_out, void* out, void* q, void* scale,
