@@ -348,8 +348,8 @@ int ta_trainer_create(ta_ctx* ctx, const ta_model_config* model, const ta_adapte
 /* The same with the activations that the forward keeps for the backward in `act_bits` bits: 16 (ta_trainer_create), or 8: the two
  * norms' rows, gate and up of every layer are held as described at TA_Q8_BLOCK and the backward reads them from there (act is
  * formed again); the residual stream, normed inputs, gate, up and act in BF16 are one layer's buffers.  Q, K, V and the attention
- * output stay in BF16.  At 7B shapes with micro-batches of 4 x 4096 tokens a trainer takes 52 GB instead of 94, a step 2 to 3 %
- * more time.  Gradients and centroid sums carry e4m3's rounding (2^-4 at most, 2.5e-2 in the mean square, of each input of a
+ * output stay in BF16.  At 7B shapes with micro-batches of 4 x 4096 tokens a trainer takes 52 GB instead of 94, a step 2 % more
+ * time.  Gradients and centroid sums carry e4m3's rounding (2^-4 at most, 2.5e-2 in the mean square, of each input of a
  * layer's backward), the forward and the loss do not.  "l<i>.cache.x_normed", ".r_in" and ".r_mid" cannot be read then, and the
  * option "fuse_swiglu" has no effect.  No reference counterpart. */
 int ta_trainer_create_ex(ta_ctx* ctx, const ta_model_config* model, const ta_adapter_config* adapter, int micro_batch,
