@@ -297,9 +297,27 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) add_rms_norm_q8_fwd_ker
     }
 }
 
+// Eight values as four pairs
+__device__ __forceinline__ void pairs(const uint4& u, uint64_t (&f)[4]) {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; i++) {
+        const float2 t = unpack_bf16x2(w[i]);
+        f[i] = pack_f32x2(t.x, t.y);
+    }
+}
+__device__ __forceinline__ void codes(const uint2& q, uint64_t (&f)[4]) {
+    float v[8];
+    widen4(q.x, 1.f, v);
+    widen4(q.y, 1.f, v + 4);
+#pragma unroll
+    for (int i = 0; i < 4; i++) f[i] = pack_f32x2(v[2 * i], v[2 * i + 1]);
+}
+
 // dx = rms * (w*dy - n * mean(w*dy*n)) (+ add_to), n from 8 bits
+// (The second bound 1 has the compiler take 166 registers at eight vectors a thread: 154 us at 8192 columns, with its own 156 160.)
 template <int TPR, int NV>
-__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) rms_norm_q8_bwd_kernel(const uint4* dy, const uint2* __restrict__ q,
+__global__ void __launch_bounds__(TPR == 32 ? 128 : TPR, NV == 8 ? 1 : 0) rms_norm_q8_bwd_kernel(const uint4* dy, const uint2* __restrict__ q,
                                                                                 const uint8_t* __restrict__ scale, const uint4* __restrict__ w,
                                                                                 const float* __restrict__ rms_saved, uint4* dx,
                                                                                 const uint4* add_to, int rows, int D) {
@@ -328,41 +346,51 @@ __global__ void __launch_bounds__(TPR == 32 ? 128 : TPR) rms_norm_q8_bwd_kernel(
 #pragma unroll
         for (int j = 0; j < NV; j++) wv[j] = lane + j * TPR < nvec ? __ldg(w + lane + j * TPR) : make_uint4(0, 0, 0, 0);
     }
-    auto weight = [&](int j, float (&f)[8]) {
-        if constexpr (kEarly) unpack8(wv[j], f);
-        else unpack8(__ldg(w + lane + j * TPR), f);
+    // Pairs of columns, two to an instruction (one by one: 43.0 -> 45.3 us at 16384 x 2048, 154 -> 188 at 8192).  n = q * 2^k: the
+    // block's power of two is taken once a vector, of the sum and of corr.
+    auto weight = [&](int j, uint64_t (&f)[4]) {
+        if constexpr (kEarly) pairs(wv[j], f);
+        else pairs(__ldg(w + lane + j * TPR), f);
     };
     float dot = 0.f;
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int i = lane + j * TPR;
         if (i >= nvec) continue;
-        float fd[8], fn[8], fw[8];
-        unpack8(d[j], fd);
-        widen8(n[j], b[j], fn);
+        uint64_t fd[4], fq[4], fw[4], acc = 0;
+        pairs(d[j], fd);
+        codes(n[j], fq);
         weight(j, fw);
 #pragma unroll
-        for (int e = 0; e < 8; e++) dot += fd[e] * fw[e] * fn[e];
+        for (int e = 0; e < 4; e++) acc = ffma2(fmul2(fd[e], fw[e]), fq[e], acc);
+        const float2 t = unpack_f32x2(acc);
+        dot += (t.x + t.y) * q8_step(b[j]);
     }
     dot = row_sum<TPR>(dot, red);
     const float corr = dot / float(D);
+    const uint64_t rms2 = pack_f32x2(rms, rms);
+    // d and n are widened again below: held as pairs they would take twice the registers
+#pragma unroll
+    for (int j = 0; j < NV; j++) asm volatile("" : "+r"(d[j].x), "+r"(d[j].y), "+r"(d[j].z), "+r"(d[j].w), "+r"(n[j].x), "+r"(n[j].y));
 #pragma unroll
     for (int j = 0; j < NV; j++) {
         const int i = lane + j * TPR;
         if (i >= nvec) continue;
-        float fd[8], fn[8], fw[8], o[8];
-        unpack8(d[j], fd);
-        widen8(n[j], b[j], fn);
+        uint64_t fd[4], fq[4], fw[4], fa[4];
+        pairs(d[j], fd);
+        codes(n[j], fq);
         weight(j, fw);
+        pairs(a[j], fa);      // zeros without add_to; one rounding to BF16, at the store
+        const float c = -corr * q8_step(b[j]);
+        const uint64_t c2 = pack_f32x2(c, c);
+        uint4 o;
+        uint32_t* ow = &o.x;
 #pragma unroll
-        for (int e = 0; e < 8; e++) o[e] = rms * (fw[e] * fd[e] - fn[e] * corr);
-        if (add_to) {
-            float fa[8];
-            unpack8(a[j], fa);
-#pragma unroll
-            for (int e = 0; e < 8; e++) o[e] += fa[e];   // one rounding, at the store
+        for (int e = 0; e < 4; e++) {
+            const float2 t = unpack_f32x2(ffma2(rms2, ffma2(fq[e], c2, fmul2(fd[e], fw[e])), fa[e]));
+            ow[e] = pack_bf16x2(t.x, t.y);
         }
-        dx[at + i] = pack8(o);
+        dx[at + i] = o;
     }
 }
 
@@ -479,14 +507,15 @@ int ta_silu_mul_q8_bwd(ta_ctx* ctx, const void* dout, const void* gate_q, const 
     });
 }
 
-// Threads a row and vectors a thread by the row's length, each the fastest of those measured on 16384 rows (us, forward / backward
-// at the longest row of the class; in parentheses the next best): 64 x 2 at 1024 columns 26.9 / 22.7 (a warp 28.3 / 25.0), 128 x 2
-// at 2048 49.4 / 39.6 (64 x 4 49.8 / 42.3), 128 x 4 at 3584 83.6 / 67.3 (256 x 2 82.8 / 70.1), at 8192 forward 256 x 4 183 (128 x 8
-// 185) and backward, which holds three arrays, 128 x 8 154 (256 x 4 168).
+// Threads a row and vectors a thread by the row's length, each the fastest of those measured on 16384 rows at the longest row of the
+// class (us; in parentheses the next best).  Forward: 64 x 2 at 1024 columns 26.9 (a warp 28.3), 128 x 2 at 2048 49.4 (64 x 4 49.8), 128
+// x 4 at 3584 83.6 (256 x 2 82.8), 256 x 4 at 8192 183 (128 x 8 185).  Backward, which holds three arrays (a call, L2 cold): 64 x 2 at
+// 1024 24.6, 128 x 2 at 2048 43.0, 256 x 2 at 4096 75.9 (128 x 4 86), 128 x 8 at 8192 154 (256 x 4 172, 512 x 2 184), 512 x 4 at 16384
+// 389 (256 x 8 516).
 // Few rows, up to four an SM, leave most of the device idle and are bound by a row's own latency: more threads a row then (us,
 // forward / backward, from L2: 1 x 896 1.7 / 1.5, with the others 2.1 / 1.6; 256 x 3584 2.9 / 2.8, 3.8 / 3.3; 64 x 8192 3.2 / 2.8, 3.8 /
 // 4.5; 592 x 8192 11.3 / 10.0, 9.6 / 14.3; beyond, at 1024 x 3584, 8.8 / 7.0, 7.8 / 8.7).
-#define TA_NORM_CASES(LAUNCH, AT_8192, AT_16384)                                        \
+#define TA_NORM_CASES(LAUNCH, AT_4096, AT_8192, AT_16384)                               \
     do {                                                                                \
         const int nvec = D / 8;                                                         \
         const bool few = rows <= 4 * ctx->sm_count;                                     \
@@ -494,7 +523,7 @@ int ta_silu_mul_q8_bwd(ta_ctx* ctx, const void* dout, const void* gate_q, const 
         else if (nvec <= 64)   LAUNCH(32, 2);                                           \
         else if (nvec <= 128)  { if (few) LAUNCH(128, 1); else LAUNCH(64, 2); }         \
         else if (nvec <= 256)  { if (few) LAUNCH(256, 1); else LAUNCH(128, 2); }        \
-        else if (nvec <= 512)  { if (few) LAUNCH(512, 1); else LAUNCH(128, 4); }        \
+        else if (nvec <= 512)  { if (few) LAUNCH(512, 1); else LAUNCH AT_4096; }        \
         else if (nvec <= 1024) { if (few) LAUNCH(512, 2); else LAUNCH AT_8192; }        \
         else                   { if (few) LAUNCH(512, 4); else LAUNCH AT_16384; }       \
     } while (0)
@@ -514,7 +543,7 @@ int ta_add_rms_norm_q8_fwd(ta_ctx* ctx, const void* x, const void* delta, const 
     const auto S = static_cast<uint8_t*>(scale);
 #define TA_LAUNCH(TPR, NV) \
     add_rms_norm_q8_fwd_kernel<TPR, NV><<<TPR == 32 ? (rows - 1) / 4 + 1 : rows, TPR == 32 ? 128 : TPR, 0, s>>>(X, De, W, R, O, Q, S, rms_out, rows, D, 1.0 / D, eps)
-    TA_NORM_CASES(TA_LAUNCH, (256, 4), (256, 8));
+    TA_NORM_CASES(TA_LAUNCH, (128, 4), (256, 4), (256, 8));
 #undef TA_LAUNCH
     TA_LAUNCH_CHECK(ctx, "add_rms_norm_q8_fwd_kernel");
     return TA_OK;
@@ -533,7 +562,7 @@ int ta_rms_norm_q8_bwd(ta_ctx* ctx, const void* dy, const void* q, const void* s
     const auto DX = static_cast<uint4*>(dx);
 #define TA_LAUNCH(TPR, NV) \
     rms_norm_q8_bwd_kernel<TPR, NV><<<TPR == 32 ? (rows - 1) / 4 + 1 : rows, TPR == 32 ? 128 : TPR, 0, s>>>(DY, Q, S, W, rms_saved, DX, AT, rows, D)
-    TA_NORM_CASES(TA_LAUNCH, (128, 8), (512, 4));
+    TA_NORM_CASES(TA_LAUNCH, (256, 2), (128, 8), (512, 4));
 #undef TA_LAUNCH
     TA_LAUNCH_CHECK(ctx, "rms_norm_q8_bwd_kernel");
     return TA_OK;
