@@ -507,15 +507,16 @@ int ta_silu_mul_q8_bwd(ta_ctx* ctx, const void* dout, const void* gate_q, const 
     });
 }
 
-// Threads a row and vectors a thread by the row's length, each the fastest of those measured on 16384 rows at the longest row of the
-// class (us; in parentheses the next best).  Forward: 64 x 2 at 1024 columns 26.9 (a warp 28.3), 128 x 2 at 2048 49.4 (64 x 4 49.8), 128
-// x 4 at 3584 83.6 (256 x 2 82.8), 256 x 4 at 8192 183 (128 x 8 185).  Backward, which holds three arrays (a call, L2 cold): 64 x 2 at
-// 1024 24.6, 128 x 2 at 2048 43.0, 256 x 2 at 4096 75.9 (128 x 4 86), 128 x 8 at 8192 154 (256 x 4 172, 512 x 2 184), 512 x 4 at 16384
-// 389 (256 x 8 516).
+// Threads a row and vectors a thread by the row's length, each the fastest of those measured on 16384 rows (us a call, L2 cold; in
+// parentheses the next best).  Forward: 64 x 2 to 1024 columns 30.7, 128 x 2 to 2048 53, 128 x 3 at 2560 65.6 (192 x 2 69.6, 128 x 4 71),
+// 128 x 4 at 3584 86 (256 x 2 as much), 256 x 3 at 5120 125 (384 x 2 135, 256 x 4 141), 256 x 4 to 8192 186 (128 x 8 188).  Backward,
+// which holds three arrays: 64 x 2 to 1024 24.6, 128 x 2 to 2048 43, 192 x 2 at 2560 55 (128 x 3 57, 256 x 2 59), 256 x 2 at 3584 70 (128 x
+// 4 80), 384 x 2 at 5120 106 (256 x 3 110, 128 x 8 119), 128 x 8 to 8192 154 (256 x 4 172, 512 x 2 184), 512 x 4 to 16384 389 (256 x 8
+// 516).  As many warps as a row needs, a number known at launch, costs the constant offsets: 28.6 at 1024, 80 at 3584.
 // Few rows, up to four an SM, leave most of the device idle and are bound by a row's own latency: more threads a row then (us,
 // forward / backward, from L2: 1 x 896 1.7 / 1.5, with the others 2.1 / 1.6; 256 x 3584 2.9 / 2.8, 3.8 / 3.3; 64 x 8192 3.2 / 2.8, 3.8 /
 // 4.5; 592 x 8192 11.3 / 10.0, 9.6 / 14.3; beyond, at 1024 x 3584, 8.8 / 7.0, 7.8 / 8.7).
-#define TA_NORM_CASES(LAUNCH, AT_4096, AT_8192, AT_16384)                               \
+#define TA_NORM_CASES(LAUNCH, AT_384, AT_512, AT_768, AT_1024, AT_2048)                 \
     do {                                                                                \
         const int nvec = D / 8;                                                         \
         const bool few = rows <= 4 * ctx->sm_count;                                     \
@@ -523,9 +524,11 @@ int ta_silu_mul_q8_bwd(ta_ctx* ctx, const void* dout, const void* gate_q, const 
         else if (nvec <= 64)   LAUNCH(32, 2);                                           \
         else if (nvec <= 128)  { if (few) LAUNCH(128, 1); else LAUNCH(64, 2); }         \
         else if (nvec <= 256)  { if (few) LAUNCH(256, 1); else LAUNCH(128, 2); }        \
-        else if (nvec <= 512)  { if (few) LAUNCH(512, 1); else LAUNCH AT_4096; }        \
-        else if (nvec <= 1024) { if (few) LAUNCH(512, 2); else LAUNCH AT_8192; }        \
-        else                   { if (few) LAUNCH(512, 4); else LAUNCH AT_16384; }       \
+        else if (nvec <= 384)  { if (few) LAUNCH(512, 1); else LAUNCH AT_384; }         \
+        else if (nvec <= 512)  { if (few) LAUNCH(512, 1); else LAUNCH AT_512; }         \
+        else if (nvec <= 768)  { if (few) LAUNCH(512, 2); else LAUNCH AT_768; }         \
+        else if (nvec <= 1024) { if (few) LAUNCH(512, 2); else LAUNCH AT_1024; }        \
+        else                   { if (few) LAUNCH(512, 4); else LAUNCH AT_2048; }        \
     } while (0)
 
 int ta_add_rms_norm_q8_fwd(ta_ctx* ctx, const void* x, const void* delta, const void* w, void* res_out, void* out, void* q, void* scale,
@@ -543,7 +546,7 @@ int ta_add_rms_norm_q8_fwd(ta_ctx* ctx, const void* x, const void* delta, const 
     const auto S = static_cast<uint8_t*>(scale);
 #define TA_LAUNCH(TPR, NV) \
     add_rms_norm_q8_fwd_kernel<TPR, NV><<<TPR == 32 ? (rows - 1) / 4 + 1 : rows, TPR == 32 ? 128 : TPR, 0, s>>>(X, De, W, R, O, Q, S, rms_out, rows, D, 1.0 / D, eps)
-    TA_NORM_CASES(TA_LAUNCH, (128, 4), (256, 4), (256, 8));
+    TA_NORM_CASES(TA_LAUNCH, (128, 3), (128, 4), (256, 3), (256, 4), (256, 8));
 #undef TA_LAUNCH
     TA_LAUNCH_CHECK(ctx, "add_rms_norm_q8_fwd_kernel");
     return TA_OK;
@@ -562,7 +565,7 @@ int ta_rms_norm_q8_bwd(ta_ctx* ctx, const void* dy, const void* q, const void* s
     const auto DX = static_cast<uint4*>(dx);
 #define TA_LAUNCH(TPR, NV) \
     rms_norm_q8_bwd_kernel<TPR, NV><<<TPR == 32 ? (rows - 1) / 4 + 1 : rows, TPR == 32 ? 128 : TPR, 0, s>>>(DY, Q, S, W, rms_saved, DX, AT, rows, D)
-    TA_NORM_CASES(TA_LAUNCH, (256, 2), (128, 8), (512, 4));
+    TA_NORM_CASES(TA_LAUNCH, (192, 2), (256, 2), (384, 2), (128, 8), (512, 4));
 #undef TA_LAUNCH
     TA_LAUNCH_CHECK(ctx, "rms_norm_q8_bwd_kernel");
     return TA_OK;
