@@ -508,11 +508,12 @@ int ta_silu_mul_q8_bwd(ta_ctx* ctx, const void* dout, const void* gate_q, const 
 }
 
 // Threads a row and vectors a thread by the row's length, each the fastest of those measured on 16384 rows (us a call, L2 cold; in
-// parentheses the next best).  Forward: 64 x 2 to 1024 columns 30.7, 128 x 2 to 2048 53, 128 x 3 at 2560 65.6 (192 x 2 69.6, 128 x 4 71),
-// 128 x 4 at 3584 86 (256 x 2 as much), 256 x 3 at 5120 125 (384 x 2 135, 256 x 4 141), 256 x 4 to 8192 186 (128 x 8 188).  Backward,
-// which holds three arrays: 64 x 2 to 1024 24.6, 128 x 2 to 2048 43, 192 x 2 at 2560 55 (128 x 3 57, 256 x 2 59), 256 x 2 at 3584 70 (128 x
-// 4 80), 384 x 2 at 5120 106 (256 x 3 110, 128 x 8 119), 128 x 8 to 8192 154 (256 x 4 172, 512 x 2 184), 512 x 4 to 16384 389 (256 x 8
-// 516).  As many warps as a row needs, a number known at launch, costs the constant offsets: 28.6 at 1024, 80 at 3584.
+// parentheses the next best).  Forward: 64 x 2 to 1024 columns 30.7, 96 x 2 at 1536 41.0 (128 x 2 43.0), 128 x 2 to 2048 53, 128 x
+// 3 at 2560 65.6 (192 x 2 69.6, 128 x 4 71), 128 x 4 at 3584 86 (256 x 2 as much), 256 x 3 at 5120 125 (384 x 2 135, 256 x 4 141),
+// 256 x 4 to 8192 186 (128 x 8 188).  Backward, which holds three arrays: 64 x 2 to 1024 24.6, 96 x 2 at 1536 32.8 (128 x 2 34.8),
+// 128 x 2 to 2048 43, 192 x 2 at 2560 55 (128 x 3 57, 256 x 2 59), 256 x 2 at 3584 70 (128 x 4 80), 384 x 2 at 5120 106 (256 x 3
+// 110, 128 x 8 119), 128 x 8 to 8192 154 (256 x 4 172, 512 x 2 184), 512 x 4 to 16384 389 (256 x 8 516).  As many warps as a row
+// needs, a number known at launch, costs the constant offsets: 28.6 at 1024, 80 at 3584.
 // Few rows, up to four an SM, leave most of the device idle and are bound by a row's own latency: more threads a row then (us,
 // forward / backward, from L2: 1 x 896 1.7 / 1.5, with the others 2.1 / 1.6; 256 x 3584 2.9 / 2.8, 3.8 / 3.3; 64 x 8192 3.2 / 2.8, 3.8 /
 // 4.5; 592 x 8192 11.3 / 10.0, 9.6 / 14.3; beyond, at 1024 x 3584, 8.8 / 7.0, 7.8 / 8.7).
@@ -523,6 +524,7 @@ int ta_silu_mul_q8_bwd(ta_ctx* ctx, const void* dout, const void* gate_q, const 
         if (nvec <= 32)        LAUNCH(32, 1);                                           \
         else if (nvec <= 64)   LAUNCH(32, 2);                                           \
         else if (nvec <= 128)  { if (few) LAUNCH(128, 1); else LAUNCH(64, 2); }         \
+        else if (nvec <= 192)  { if (few) LAUNCH(256, 1); else LAUNCH(96, 2); }         \
         else if (nvec <= 256)  { if (few) LAUNCH(256, 1); else LAUNCH(128, 2); }        \
         else if (nvec <= 384)  { if (few) LAUNCH(512, 1); else LAUNCH AT_384; }         \
         else if (nvec <= 512)  { if (few) LAUNCH(512, 1); else LAUNCH AT_512; }         \

@@ -170,7 +170,7 @@ def test_offsets_past_32_bits(ctx):
 NORM_SHAPES = [(1, 8), (3, 40), (5, 248), (4, 256), (6, 264), (9, 512), (130, 896), (33, 904), (2, 1024), (2, 1032), (17, 1536), (5, 2048),
                (5, 2056), (3, 3584), (2, 4096), (2, 4104), (3, 8192), (2, 8200), (2, 16384),
                # and more rows than four an SM, which take other variants
-               (2000, 248), (700, 904), (601, 1536), (640, 2056), (650, 3584), (600, 4104), (600, 8192), (600, 8200)]
+               (2000, 248), (700, 904), (601, 1536), (620, 1544), (640, 2056), (650, 3584), (600, 4104), (600, 8192), (600, 8200)]
 
 
 def sum_err(D):
