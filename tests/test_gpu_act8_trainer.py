@@ -78,6 +78,36 @@ def test_micro_batches_and_a_second_step(ctx):
     assert rel(parts["flat"], whole["flat"]) <= 2e-2 and abs(parts["loss"] - whole["loss"]) <= 1e-4 * whole["loss"]
 
 
+@pytest.mark.parametrize("rank", [8, 64, 200])
+def test_ranks(ctx, rank):
+    """Groups of adapters side by side up to 3 x 208 ranks, which gA takes in passes."""
+    cfg = rc.tiny_cfg(hidden=256, hq=4, hkv=2, hd=64, inter=712, layers=1)
+    B, T = 2, 96
+    base, adapter, toks, tgts = rc.make_case(cfg, B, T, rank, targets=NAMES, seed=17, std=0.02, b_std=0.02)
+    a = run(ctx, cfg, base, adapter, toks, tgts, B, T, 8, 127, rank=rank)
+    b = run(ctx, cfg, base, adapter, toks, tgts, B, T, 16, 127, rank=rank)
+    assert abs(a["loss"] - b["loss"]) <= 1e-4 * b["loss"]
+    for k in b["grads"]:
+        assert rel(a["grads"][k], b["grads"][k]) <= REL, k
+
+
+def test_fused_swiglu_option_has_no_effect(ctx):
+    from tensor_adapt_b200.trainer import AdaptTrainer, AdapterConfig
+    cfg = rc.tiny_cfg(hidden=256, hq=4, hkv=2, hd=64, inter=512, layers=2)
+    B, T = 2, 128
+    base, adapter, toks, tgts = rc.make_case(cfg, B, T, 16, targets=NAMES, seed=5, std=0.02, b_std=0.02)
+    flat = []
+    for fused in (-1, 0, 1):
+        tr = AdaptTrainer(ctx, rc.model_config(cfg), AdapterConfig.defaults(rank=16, targets=127), B, T, act_bits=8)
+        tr._call("ta_trainer_set_option", b"fuse_swiglu", fused)
+        rc.load_into_trainer(tr, cfg, base, adapter)
+        tr.zero_grad()
+        tr.forward_backward(toks[0], tgts[0], B)
+        flat.append(tr.download("lora.grad"))
+        tr.close()
+    assert np.array_equal(flat[0], flat[1]) and np.array_equal(flat[0], flat[2])
+
+
 def test_activation_memory(ctx):
     import torch
     from tensor_adapt_b200.trainer import AdaptTrainer, AdapterConfig
