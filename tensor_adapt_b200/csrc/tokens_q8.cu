@@ -423,26 +423,30 @@ struct Call {
     int accumulate;
 };
 
-// Clusters of 1, 2, 4, 8 and 16 CTAs that the device holds at a time, asked once for each kernel and device.  The answer counts one CTA
-// an SM for these kernels, two of which run on one (NB <= 64: counters show 24 warps active of 2 x 12); clusters of cs at two CTAs an
-// SM are then as many as clusters of cs / 2 at one.
-constexpr int kSizes = 5;
+// Clusters of 1 to 16 CTAs that the device holds at a time with one CTA on an SM (`alone`) and in all, asked once for each kernel and
+// device.  The answer counts one CTA an SM for these kernels, two of which run on one (NB <= 64: counters show 24 warps active of 2 x
+// 12); clusters of cs at two CTAs an SM are then as many as clusters of cs / 2 at one.  Above 8 that did not hold: 12 clusters of 16 take
+// 13.5 us at 1536 columns x 8192 tokens, of 8 11.9.
+constexpr int kMostCtas = 16;
 struct Residency {
-    int n[kSizes] = {};
+    int alone[kMostCtas + 1] = {}, all[kMostCtas + 1] = {};
     bool known = false;
 };
 std::mutex residency_lock;   // contexts of several host threads share the answers
 template <typename F>
 void ask(F kernel, cudaLaunchConfig_t cfg, cudaLaunchAttribute& at, int per_sm, int sm_count, Residency& r) {
-    int n[kSizes];
-    for (int k = 0; k < kSizes; k++) {
-        at.val.clusterDim.x = 1u << k;
-        cfg.gridDim = dim3(1u << k);
-        if (cudaOccupancyMaxActiveClusters(&n[k], kernel, &cfg) != cudaSuccess) n[k] = 0;
+    int n[kMostCtas + 1] = {};
+    for (int cs = 1; cs <= kMostCtas; cs++) {
+        at.val.clusterDim.x = unsigned(cs);
+        cfg.gridDim = dim3(unsigned(cs));
+        if (cudaOccupancyMaxActiveClusters(&n[cs], kernel, &cfg) != cudaSuccess) n[cs] = 0;
     }
     (void)cudaGetLastError();
-    const bool halved = per_sm == 2 && n[0] <= sm_count;
-    for (int k = 0; k < kSizes; k++) r.n[k] = !halved ? n[k] : k == 0 ? 2 * n[0] : n[k] > 0 ? n[k - 1] : 0;
+    const bool both = n[1] > sm_count;      // it did count two
+    for (int cs = 1; cs <= kMostCtas; cs++) {
+        r.alone[cs] = both ? n[cs] / 2 : n[cs];
+        r.all[cs] = both || per_sm == 1 || cs > 8 ? n[cs] : cs == 1 ? 2 * n[1] : std::max(n[cs], n[(cs + 1) / 2]);
+    }
     r.known = true;
 }
 
@@ -472,17 +476,19 @@ int launch(const Call& c) {
         }
         fit = known;
     }
-    // CTAs on a column tile: the fewest rounds of clusters x chunks of a CTA, with what a CTA costs whatever its chunks (8 us, 11 in
-    // a cluster of 16; a chunk takes 0.9).  16 against 8, us: 512 columns x 16384 tokens 12.4 / 16.8, 896 x 8192 10.4 / 11.9, 896 x
-    // 2048 7.6 / 7.4, 1536 x 4096 10.7 / 9.0.
+    // CTAs on a column tile: the least time by what was measured (us): 6 whatever the chunks, 7 in a cluster above 8, and a CTA's chunk
+    // 0.72 alone on its SM, 1.05 with another.  E.g. 8192 tokens: 896 columns (7 tiles) 16 CTAs a tile 10.0 (8: 11.9); 1536, 8 11.9 (6
+    // 13.7, 16 13.5); 4864, 6 16.6 (4 20.3, 8 23.2); 8960, 4 24.8 (2 29.6, 8 41).
     const unsigned tiles = (unsigned(c.N) + kFeat - 1) / kFeat, rows = (unsigned(c.M) + NB - 1) / NB;
     const int chunks = (c.K + kTok - 1) / kTok;
+    const long clusters = long(tiles) * rows;
     int cs = 0;
     long least = 0;
-    for (int k = 0; k < kSizes && (1 << k) <= chunks; k++) {
-        if (fit.n[k] <= 0) continue;
-        const long rounds = (long(tiles) * rows + fit.n[k] - 1) / fit.n[k], cost = rounds * (((chunks - 1) >> k) + 1 + (k == 4 ? 11 : 8));
-        if (cs == 0 || cost < least) { least = cost; cs = 1 << k; }
+    for (int k = 1; k <= kMostCtas && k <= chunks; k++) {
+        if (fit.all[k] <= 0) continue;
+        const long rounds = (clusters + fit.all[k] - 1) / fit.all[k], mine = (chunks + k - 1) / k;
+        const long cost = rounds * ((k > 8 ? 700 : 600) + mine * (clusters > fit.alone[k] ? 105 : 72));
+        if (cs == 0 || cost < least) { least = cost; cs = k; }
     }
     if (cs == 0) return fail(ctx, TA_ERR_CUDA, "gemm_tokens_q8_f32: the kernel cannot be resident on this device");
     at.val.clusterDim.x = unsigned(cs);

@@ -381,7 +381,7 @@ GRADS = [(8, 8, 1), (16, 64, 16), (16, 40, 17), (24, 904, 130), (32, 72, 15), (4
          (128, 64, 300), (192, 96, 129), (256, 8, 40), (16, 18944, 260), (16, 64, 5000), (8, 64, 0),
          (16, 40, 9000), (64, 1160, 6100), (136, 72, 3300), (200, 136, 5000), (64, 128, 9001),
          (192, 64, 9000), (120, 40, 20000), (200, 24, 12345),
-         (16, 16, 100), (24, 32, 1), (32, 48, 129), (40, 16, 8), (768, 64, 300), (8, 48, 70000), (32, 4864, 640), (64, 8, 131)]
+         (16, 16, 100), (24, 32, 1), (32, 48, 129), (40, 16, 8), (768, 64, 300), (8, 48, 70000), (32, 4864, 640), (64, 8, 131), (24, 2048, 3000), (128, 4864, 900), (16, 512, 384)]
 
 
 def grad_case(rng, M, N, K, size=1.0):
