@@ -37,7 +37,7 @@ namespace {
 namespace cg = cooperative_groups;
 
 constexpr int kFeat = 128, kTok = 128;      // a chunk: columns of q, tokens
-constexpr int kConv = 8;                    // warps that widen q, in two sets; behind them loaders of q, one of A, one that multiplies
+constexpr int kConv = 8;                    // warps that widen q, in two sets; behind them the loaders, one that issues TMA copies, one that multiplies
 constexpr int kPitch = kFeat + 4;           // of the sums in shared memory
 
 constexpr int kRun = 4;                     // chunks that D takes in a row
